@@ -7,6 +7,7 @@ list is not used.
 
 import glob
 import os
+import subprocess
 
 from setuptools import setup
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension
@@ -30,6 +31,19 @@ nvcc_flags = [
 if os.environ.get("TITANS_PTXAS_VERBOSE") == "1":
     nvcc_flags.append("-Xptxas=-v")
 
+
+
+def shared_libstdcxx():
+    """Link libstdc++ as a shared library where the compiler finds it, also if its default is the static one:
+    two copies in one process (the other is torch's) crash as soon as an error message formats a number."""
+    cxx = os.environ.get("CXX", "c++").split()
+    try:
+        path = subprocess.run(cxx + ["-print-file-name=libstdc++.so.6"], capture_output=True, text=True).stdout.strip()
+    except OSError:
+        return []
+    return [path] if os.path.isabs(path) else []
+
+
 setup(
     name="titans_pytorch_b200",
     version="0.1.0",
@@ -39,6 +53,7 @@ setup(
             name="titans_pytorch_b200._C",
             sources=sources,
             include_dirs=[os.path.join(HERE, CSRC)],
+            extra_link_args=shared_libstdcxx(),
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": nvcc_flags},
         )
     ],
