@@ -98,6 +98,32 @@ void gemm_sm100(const at::Tensor& A, bool a_mn, const at::Tensor& B, bool b_mn, 
                 int64_t mode, const at::Tensor& Cout, const c10::optional<at::Tensor>& R,
                 const c10::optional<at::Tensor>& C2, const c10::optional<at::Tensor>& R2,
                 const c10::optional<at::Tensor>& gates, double scale, int64_t act, int64_t ffn_f, int64_t splits);
+// rope.cu
+at::Tensor rotary_embedding(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& freq, bool half,
+                            double amplitude, bool backward);
+// kv_cache.cu
+at::Tensor kv_cache_write(at::Tensor& ck, at::Tensor& cv, const c10::optional<at::Tensor>& ks,
+                          const c10::optional<at::Tensor>& vs, const at::Tensor& k, const at::Tensor& v,
+                          const at::Tensor& start, const c10::optional<at::Tensor>& count,
+                          const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& freq, bool half,
+                          double amplitude, int64_t offset);
+std::vector<at::Tensor> kv_cache_read(const at::Tensor& ck, const at::Tensor& cv,
+                                      const c10::optional<at::Tensor>& ks, const c10::optional<at::Tensor>& vs,
+                                      const at::Tensor& lengths, int64_t n, at::ScalarType dtype);
+// decode_attn.cu
+std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv,
+                                         const c10::optional<at::Tensor>& ks, const c10::optional<at::Tensor>& vs,
+                                         const at::Tensor& lengths, const c10::optional<at::Tensor>& pk,
+                                         const c10::optional<at::Tensor>& pv, int64_t window, double scale,
+                                         bool want_lse);
+// sampling.cu
+std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const at::Tensor& u,
+                                      const c10::optional<at::Tensor>& temp, double temp0,
+                                      const c10::optional<at::Tensor>& top_k, int64_t top_k0,
+                                      const c10::optional<at::Tensor>& top_p, double top_p0,
+                                      const c10::optional<at::Tensor>& min_p, double min_p0,
+                                      const c10::optional<at::Tensor>& penalty, double penalty0,
+                                      const c10::optional<at::Tensor>& seen);
 }  // namespace tb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -169,6 +195,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("R2") = pybind11::none(), pybind11::arg("gates") = pybind11::none(),
         pybind11::arg("scale") = 1.0, pybind11::arg("act") = 0, pybind11::arg("ffn_f") = 0,
         pybind11::arg("splits") = 0);
+  m.def("rotary_embedding", &tb::rotary_embedding);
+  m.def("kv_cache_write", &tb::kv_cache_write);
+  m.def("kv_cache_read", &tb::kv_cache_read);
+  m.def("decode_attention", &tb::decode_attention);
+  m.def("sample_tokens", &tb::sample_tokens);
   m.def("exp2_poly_eval", &tb::exp2_poly_eval);
   m.def("kernel_error_status", &tb::kernel_error_status, pybind11::arg("device") = 0, pybind11::arg("reset") = true);
 }

@@ -1,0 +1,181 @@
+// Rotary positions, forward and backward (the same rotation by the opposite
+// angle).  x [B, T, H, d] with any strides over B, T, H; the first 2n of d are
+// rotated in pairs, interleaved (2i, 2i+1) or half (i, i+n), the rest copied.
+//
+// Bound by memory: x is read once and y written once.  A block takes a few
+// tokens; their cos / sin are computed once in shared memory (fp64 angle, see
+// rope.cuh) and serve every head, then each thread moves 16-byte vectors.
+#include "common.cuh"
+#include "rope.cuh"
+
+namespace tb {
+namespace {
+
+struct RopeArgs {
+  const void* x;
+  void* y;
+  const int64_t* pos;
+  const float* freq;
+  int64_t sxb, sxt, sxh, spb, spt;
+  int64_t tokens;  // B * T
+  int T, H, d, n;
+  float amplitude, sign;
+};
+
+constexpr int kThreads = 256;
+
+// Interleaved: a 16-byte vector holds whole pairs; the table is padded with
+// (1, 0) past the rotated part, so the copied tail needs no branch.
+// Half: a work item is a pair of vectors (i, i + n) or one vector of the tail.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(kThreads) rope_vec_kernel(RopeArgs a, int tok_per_block) {
+  constexpr int V = Vec16<T>::N;
+  extern __shared__ float2 tab[];  // [tok_per_block][pairs]
+  const int pairs = HALF ? a.n : a.d / 2;
+  const int64_t tok0 = (int64_t)blockIdx.x * tok_per_block;
+  const int toks = (int)min((int64_t)tok_per_block, a.tokens - tok0);
+  for (int i = threadIdx.x; i < toks * pairs; i += kThreads) {
+    const int t = i / pairs, p = i - t * pairs;
+    const int tok = (int)tok0 + t;
+    const int b = tok / a.T, tt = tok - b * a.T;
+    float2 cs = make_float2(1.f, 0.f);
+    if (p < a.n) {
+      cs = rope_cos_sin(a.pos[b * a.spb + tt * a.spt], a.freq[p], a.amplitude);
+      cs.y *= a.sign;
+    }
+    tab[i] = cs;
+  }
+  __syncthreads();
+  const int head_items = HALF ? a.n / V + (a.d - 2 * a.n) / V : a.d / V;
+  const int tok_items = a.H * head_items;
+  for (int i = threadIdx.x; i < toks * tok_items; i += kThreads) {
+    const int t = i / tok_items, r = i - t * tok_items;
+    const int h = r / head_items, v = r - h * head_items;
+    const int tok = (int)tok0 + t;
+    const int b = tok / a.T, tt = tok - b * a.T;
+    const T* x = (const T*)a.x + b * a.sxb + tt * a.sxt + h * a.sxh;
+    T* y = (T*)a.y + ((int64_t)tok * a.H + h) * a.d;
+    const float2* cs = tab + t * pairs;
+    if constexpr (HALF) {
+      if (v < a.n / V) {
+        float p[V], q[V], u[V], w[V];
+        load16<T>(x + v * V, p);
+        load16<T>(x + a.n + v * V, q);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float2 c = cs[v * V + k];
+          u[k] = p[k] * c.x - q[k] * c.y;
+          w[k] = p[k] * c.y + q[k] * c.x;
+        }
+        store16<T>(y + v * V, u);
+        store16<T>(y + a.n + v * V, w);
+      } else {
+        const int at = 2 * a.n + (v - a.n / V) * V;
+        *reinterpret_cast<uint4*>(y + at) = *reinterpret_cast<const uint4*>(x + at);
+      }
+    } else {
+      float p[V], u[V];
+      load16<T>(x + v * V, p);
+#pragma unroll
+      for (int k = 0; k < V; k += 2) {
+        const float2 c = cs[(v * V + k) / 2];
+        u[k] = p[k] * c.x - p[k + 1] * c.y;
+        u[k + 1] = p[k] * c.y + p[k + 1] * c.x;
+      }
+      store16<T>(y + v * V, u);
+    }
+  }
+}
+
+// Any size, stride and alignment: one element pair (or one tail element) per item.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rope_scalar_kernel(RopeArgs a, bool half, int64_t sxd) {
+  extern __shared__ float2 tab[];
+  const int tok = blockIdx.x;
+  const int b = tok / a.T, tt = tok - b * a.T;
+  for (int p = threadIdx.x; p < a.n; p += kThreads) {
+    float2 cs = rope_cos_sin(a.pos[b * a.spb + tt * a.spt], a.freq[p], a.amplitude);
+    cs.y *= a.sign;
+    tab[p] = cs;
+  }
+  __syncthreads();
+  const int head_items = a.d - a.n;
+  for (int i = threadIdx.x; i < a.H * head_items; i += kThreads) {
+    const int h = i / head_items, v = i - h * head_items;
+    const T* x = (const T*)a.x + b * a.sxb + tt * a.sxt + h * a.sxh;
+    T* y = (T*)a.y + ((int64_t)tok * a.H + h) * a.d;
+    if (v < a.n) {
+      const int i0 = half ? v : 2 * v, i1 = half ? v + a.n : 2 * v + 1;
+      const float p = to_f<T>(x[i0 * sxd]), q = to_f<T>(x[i1 * sxd]);
+      const float2 c = tab[v];
+      y[i0] = from_f<T>(p * c.x - q * c.y);
+      y[i1] = from_f<T>(p * c.y + q * c.x);
+    } else {
+      y[v + a.n] = x[(v + a.n) * sxd];
+    }
+  }
+}
+
+}  // namespace
+
+at::Tensor rotary_embedding(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& freq, bool half,
+                            double amplitude, bool backward) {
+  TB_CHECK_CUDA(x);
+  TORCH_CHECK(x.dim() == 4, "rotary_embedding: x must be [B, T, H, d]");
+  TORCH_CHECK(pos.device() == x.device() && freq.device() == x.device(),
+              "rotary_embedding: x, positions and inv_freq must be on one device");
+  TORCH_CHECK(pos.scalar_type() == at::kLong && freq.scalar_type() == at::kFloat && freq.dim() == 1 &&
+                  freq.is_contiguous(),
+              "rotary_embedding: int64 positions and a contiguous fp32 inv_freq");
+  const int64_t B = x.size(0), T = x.size(1), H = x.size(2), d = x.size(3), n = freq.numel();
+  TORCH_CHECK(2 * n <= d, "rotary_embedding: ", n, " frequencies rotate ", 2 * n, " of only ", d, " dimensions");
+  TORCH_CHECK(d <= 1024 && H <= (1 << 20) && T < (1ll << 31), "rotary_embedding: at most 1024 dimensions a head");
+  TORCH_CHECK((pos.dim() == 1 && pos.size(0) == T) || (pos.dim() == 2 && pos.size(0) == B && pos.size(1) == T),
+              "rotary_embedding: positions must be [T] or [B, T]");
+  const at::cuda::CUDAGuard g(x.device());
+  at::Tensor y = at::empty({B, T, H, d}, x.options());
+  if (y.numel() == 0) return y;
+  RopeArgs a;
+  a.x = x.data_ptr();
+  a.y = y.data_ptr();
+  a.pos = pos.data_ptr<int64_t>();
+  a.freq = freq.data_ptr<float>();
+  a.sxb = x.stride(0);
+  a.sxt = x.stride(1);
+  a.sxh = x.stride(2);
+  a.spb = pos.dim() == 2 ? pos.stride(0) : 0;
+  a.spt = pos.stride(-1);
+  a.tokens = B * T;
+  TORCH_CHECK(a.tokens < (1ll << 31), "rotary_embedding: too many tokens in one call");
+  a.T = (int)T;
+  a.H = (int)H;
+  a.d = (int)d;
+  a.n = (int)n;
+  a.amplitude = (float)amplitude;
+  a.sign = backward ? -1.f : 1.f;
+  TB_DISPATCH_FLOAT(x.scalar_type(), "rotary_embedding", [&] {
+    constexpr int V = Vec16<scalar_t>::N;
+    const bool vec = (x.stride(3) == 1 || d == 1) && d % V == 0 && aligned16(x) && a.sxb % V == 0 &&
+                     a.sxt % V == 0 && a.sxh % V == 0 && (!half || n % V == 0);
+    if (!vec) {
+      rope_scalar_kernel<scalar_t><<<(unsigned)a.tokens, kThreads, n * sizeof(float2), stream()>>>(a, half,
+                                                                                                x.stride(3));
+      return;
+    }
+    // enough tokens a block for about four vectors a thread, if that still fills the GPU
+    const int64_t items = H * d / V;
+    int64_t per = std::max<int64_t>(1, 4 * kThreads / items);
+    per = std::min(per, std::max<int64_t>(1, a.tokens / (num_sms() * 4)));
+    per = std::min<int64_t>(per, 16);
+    const size_t smem = per * (half ? std::max<int64_t>(n, 1) : d / 2) * sizeof(float2);
+    const unsigned blocks = (unsigned)((a.tokens + per - 1) / per);
+    if (half)
+      rope_vec_kernel<scalar_t, true><<<blocks, kThreads, smem, stream()>>>(a, (int)per);
+    else
+      rope_vec_kernel<scalar_t, false><<<blocks, kThreads, smem, stream()>>>(a, (int)per);
+  });
+  check_launch("rotary_embedding");
+  return y;
+}
+
+}  // namespace tb

@@ -18,6 +18,7 @@ import torch.nn.functional as F
 from ..config import TitansConfig
 from ..ops.linear import linear
 from ..ops.attention import prefix_window_mask, window_attention
+from ..ops.rope import rotary_embedding
 
 
 class RotaryPositionEmbedding(nn.Module):
@@ -51,6 +52,12 @@ class RotaryPositionEmbedding(nn.Module):
         cos = self.cos_cached[seq_offset:seq_offset + n]
         sin = self.sin_cached[seq_offset:seq_offset + n]
         return self._apply_rotary(q, cos, sin), self._apply_rotary(k, cos, sin)
+
+    def rotate(self, x: torch.Tensor, positions: torch.Tensor, use_kernels: bool | None = None) -> torch.Tensor:
+        """Rotate ``x`` [B, T, H, d] (any strides, no copy) at ``positions`` [T] or [B, T], differentiably and in
+        one pass, with angles that stay exact at far positions
+        (:func:`~titans_pytorch_b200.ops.rope.rotary_embedding`)."""
+        return rotary_embedding(x, positions, self.inv_freq, use_kernels=use_kernels)
 
     @staticmethod
     def _apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
