@@ -760,7 +760,7 @@ def _check_sampling(logits, u, generated=None, **kw):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("V", [1, 2, 33, 1000, 4099, 32000, 131072])
+@pytest.mark.parametrize("V", [1, 2, 33, 1000, 4099, 32000, 131072, 400001])
 @pytest.mark.parametrize("temperature,k,p,m", SAMPLE_SETTINGS)
 def test_sampling_kernel(V, dtype, temperature, k, p, m):
     _cuda()

@@ -75,7 +75,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
                   use_kernels: bool | None = None):
     """Token ids (int64 [B]) drawn from ``logits`` [B, V] with the numbers ``uniform`` (fp32 [B], in [0, 1)).
 
-    Every setting is a number or a tensor [B].  ``generated`` (int64 [B, n]):
+    Every setting is a number or a tensor [B]; V is at most 2^19.  ``generated`` (int64 [B, n]):
     tokens that ``repetition_penalty`` applies to; ids outside the vocabulary
     (padding) are passed over.  With ``return_logprob`` also the log-probability
     of each token among those kept (fp32 [B]; 0 where ``temperature <= 0``).
