@@ -11,22 +11,31 @@
 //           u * (their sum)
 // T <= 0 takes the first largest z.
 //
-// Weights are held as integers round(w * 2^F), F = 47 for vocabularies up to
-// 2^15 and less beyond so that a sum fits 62 bits: integer sums do not depend
-// on their order, so a row gives the same token whatever the split, and the
-// borders of running sums lie within 2^-47 or so of the real ones (fp32 sums
-// would move tokens).
+// Weights are held as integers round(w * 2^F): integer sums do not depend on
+// their order, so the same row always gives the same token.  F = 47 for
+// vocabularies up to 2^15, 44 at 2^17, 38 at 2^19, so that sums of V of them
+// fit; the borders of running sums are off by the square root of V such
+// roundings at most, where fp32 sums would move tokens.
 //
-// A row is a cluster of 1 to 8 blocks, each with its slice of z in shared
-// memory as order-preserving 32-bit keys: the logits are read from memory once.
-// Thresholds come from histograms, not from sorting: 1024 bins, first linear in
-// z (1/32 wide, from the maximum down), then by key within the chosen bin, until
-// a bin decides (one element, or one value).  Two passes settle nearly every
-// row.  Each pass ends in one cluster barrier, after which every block sums the
-// blocks' bins through distributed shared memory and finds the same answer.
-// What bounds it: a single row by that chain of barriers; a large batch of
-// large vocabularies by the arithmetic on every element (an fp64 exponential
-// and four shared-memory atomics).
+// Nothing is sorted.  The first pass over the row takes the maximum and counts
+// elements in 1024 bins linear in z (1/32 wide, around a sampled maximum).  From
+// the counts follow the bin of the k-th largest, or, for top-p, two bins between
+// which the border must lie (a bin's elements weigh the same within 3 %).  The
+// second pass (the row is in L2 now) sums the exact weights and moves every
+// element that may still be kept into a list in shared memory; if they do not
+// fit, later passes go on reading the row.  The list is narrowed by histograms
+// over the keys (order-preserving 32-bit images of z) until a bin decides: one
+// element, or one value.  The draw is the same search over the index: 1024
+// index bins, then the elements of one bin.
+//
+// One block does all of this for a row; while SMs are free, up to seven more
+// take parts of the two passes and add their counts, sums and list entries to
+// its shared memory, three barriers in all.  (Every block of the cluster summing
+// all blocks' bins itself cost 2.5 us a search, and sorting nothing but keeping
+// the row in shared memory gained nothing over reading it again from L2.)
+// What bounds it: one row, the chain of block barriers; many rows of large
+// vocabularies, the instructions of the two passes (about 25 of the fp64
+// exponential and 25 of loads, keys and bins per element).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -36,11 +45,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 1024;
-constexpr int kTable = 256;              // entries of the exponential's table
-constexpr int kMaxSlice = 40960;         // keys a block can hold
-constexpr int kMaxCluster = 8;
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBins = kThreads;          // one a thread
+constexpr int kTable = 16;               // entries of the exponential's table
+constexpr int kSharedLimit = 226 * 1024;
 
 // one value for every row, or one per row
 struct Setting {
@@ -52,7 +60,7 @@ struct Setting {
 struct SampleArgs {
   const void* logits;
   int64_t ls;
-  int V, slice, fbits;
+  int V, slice, fbits, limb, list_cap, index_shift;
   const float* u;
   Setting temp, top_p, min_p, penalty;
   const int64_t* top_k;
@@ -64,229 +72,304 @@ struct SampleArgs {
   float* logprob;
 };
 
+using u64 = unsigned long long;
+
 // order-preserving map of fp32 to uint32
 __device__ __forceinline__ uint32_t key_of(float z) {
   const uint32_t b = __float_as_uint(z);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 constexpr uint32_t kLowest = 0x007fffffu;  // key of -inf
 
-struct Hist {
-  uint32_t n[kBins], m0[kBins], m1[kBins], m2[kBins];  // count; weight in 16-bit limbs
-};
-
-struct Shared {
-  double table[kTable];      // 2^(j / kTable) * 2^F
-  Hist hist[2];
-  unsigned long long scan[kWarps];
-  unsigned long long best;   // this block's largest (key, index)
-  unsigned long long mass;   // this block's kept weight
-  uint32_t ties;             // this block's elements at the threshold
-  uint32_t warp_ties[kWarps];
-  unsigned long long warp_mass[kWarps];
-  int bin;
+struct __align__(16) Shared {
+  double table[kTable];  // 2^(j / kTable) * 2^F
+  uint32_t n[kBins], m0[kBins], m1[kBins], m2[kBins];  // count; weight in three limbs (shared memory adds 32 bits)
+  u64 scan[kWarps];
+  double scan_d[kWarps][2];
+  float scan_f[kWarps];
+  int bin, bin_lo, bin_hi, at;
   uint32_t bin_n;
-  unsigned long long ahead;
+  u64 ahead;
   uint32_t edge[2];
+  // of the row's first block: what the others add to, and what it tells them
+  u64 best[8], total[8];  // by block (64-bit atomics on another block's shared memory lost updates)
+  uint32_t top_key, lo;
+  int list_n, done, listing, summing;
 };
 
-__device__ __forceinline__ unsigned long long warp_sum64(unsigned long long v) {
+template <typename V> __device__ __forceinline__ V warp_scan(V v) {  // inclusive
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 1; o < 32; o <<= 1) {
+    const V x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
   return v;
 }
 
-template <typename T, bool RESIDENT>
+template <typename T>
 struct Row {
+  static constexpr int VEC = 8 / sizeof(T);
   const SampleArgs& a;
   Shared& s;
-  uint32_t* keys;       // RESIDENT: this block's slice
-  uint32_t* seen_bits;  // one bit per element of the slice
+  const uint32_t* seen_bits;
+  uint2* list;        // (key, index)
   const T* lr;
   float div, pen;
-  int row, rank, blocks, i0, n;  // the slice is [i0, i0 + n)
-  uint32_t top_key;
-  float zmax;
-  double zmax_d;
-  int level = 0;        // histogram buffers alternate
+  bool vec;           // 8-byte loads
+  bool plain;         // z is the logit
+  bool listed = false;
+  float ref = 0.f;    // upper edge of bin 0 of the first pass
+  uint32_t top_key = 0u;
+  double zmax = 0.0;
 
-  __device__ __forceinline__ uint32_t make_key(float logit, int i) const {
-    float z = __fdiv_rn(logit, div);
-    if (a.seen && (seen_bits[i >> 5] >> (i & 31) & 1u)) z = __fdiv_rn(z, pen);
-    return isnan(z) ? kLowest : key_of(z == 0.f ? 0.f : z);
+  __device__ __forceinline__ void set_top(uint32_t key) {
+    top_key = key;
+    zmax = (double)value_of(key);
   }
-  __device__ __forceinline__ uint32_t key_at(int i) const {
-    if constexpr (RESIDENT) return keys[i];
-    return make_key(to_f<T>(lr[i0 + i]), i);
-  }
-
-  __device__ __forceinline__ void cluster_sync() const {
+  static __device__ __forceinline__ void cluster_sync(int blocks) {
     if (blocks > 1)
       cg::this_cluster().sync();
     else
       __syncthreads();
   }
-  template <typename P> __device__ __forceinline__ const P* peer(const P* p, int r) const {
-    return blocks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
+
+  // z of an element: -0 becomes 0; NaN stays NaN (its key is that of -inf)
+  __device__ __forceinline__ float scaled(float logit, int i) const {
+    float z = logit;
+    if (!plain) {
+      z = __fdiv_rn(z, div);
+      if (a.seen && (seen_bits[i >> 5] >> (i & 31) & 1u)) z = __fdiv_rn(z, pen);
+    }
+    return z + 0.f;
+  }
+  static __device__ __forceinline__ uint32_t key_or_low(float z) { return isnan(z) ? kLowest : key_of(z); }
+  __device__ __forceinline__ uint32_t key_at(int i) const { return key_or_low(scaled(to_f<T>(lr[i]), i)); }
+
+  // f(z[VEC], index of the first, how many) for groups of elements of [i0, i1);
+  // the lanes of a warp call it together (none behind the end).
+  template <typename F> __device__ __forceinline__ void groups(int i0, int i1, F f) const {
+    // Short loop bodies: a pass runs over them a few times only.  Four vectors are in flight a thread.
+    constexpr int AHEAD = 4;
+    int rest = i0;
+    if (vec) {
+      const int v0 = i0 / VEC, v1 = i1 / VEC;  // i0 is a multiple of VEC
+      const uint2* src = reinterpret_cast<const uint2*>(lr);
+      uint2 x[AHEAD];
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        const int v = v0 + q * kThreads + threadIdx.x;
+        x[q] = v < v1 ? src[v] : make_uint2(0u, 0u);
+      }
+#pragma unroll 1
+      for (int b = v0; b < v1; b += kThreads) {
+        const int v = b + threadIdx.x;
+        union { uint2 raw; T e[VEC]; } cur;
+        cur.raw = x[0];
+#pragma unroll
+        for (int q = 0; q + 1 < AHEAD; ++q) x[q] = x[q + 1];
+        const int next = v + AHEAD * kThreads;
+        if (next < v1) x[AHEAD - 1] = src[next];
+        float z[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) z[k] = v < v1 ? scaled(to_f<T>(cur.e[k]), v * VEC + k) : 0.f;
+        f(z, v * VEC, v < v1 ? VEC : 0);
+      }
+      rest = v1 * VEC;
+    }
+    // the tail, and rows that are not aligned
+#pragma unroll 1
+    for (int b = rest; b < i1; b += kThreads) {
+      const int i = b + threadIdx.x;
+      float z[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) z[k] = 0.f;
+      if (i < i1) z[0] = scaled(to_f<T>(lr[i]), i);
+      f(z, i, i < i1 ? 1 : 0);
+    }
+  }
+  // f(key, index) for every element of the list, or of the row; the lanes of a warp call it together (key 0: none).
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    if (listed) {
+      const int n = s.list_n;
+#pragma unroll 1
+      for (int b = 0; b < n; b += kThreads) {
+        const int i = b + threadIdx.x;
+        const uint2 e = i < n ? list[i] : make_uint2(0u, 0u);
+        f(e.x, (int)e.y);
+      }
+    } else {
+      groups(0, a.V, [&](const float (&z)[VEC], int i, int n) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f(k < n ? key_or_low(z[k]) : 0u, i + k);
+      });
+    }
   }
 
   // exp(z - zmax) * 2^F, as a double, by the table-driven method (Tang, 1989):
-  // x = k ln2 / 256 + r, 2^(k / 256) from the table and the exponent, e^r by its
-  // series to r^4 (|r| <= 1.4e-3: 4e-17 beyond it).
+  // x = k ln2 / 16 + r, 2^(k / 16) from the table and the exponent, e^r by its
+  // series to r^6 (|r| <= 0.022: 5e-16 beyond it).  Sixteen doubles fill the
+  // shared-memory banks once, so lanes never wait for one another (a table of
+  // 256 with a shorter series did: 20 against 9 us for a row of 32000).
   __device__ __forceinline__ double weight(uint32_t key) const {
     if (key == top_key) return s.table[0];
-    const double x = (double)value_of(key) - zmax_d;
+    return weight_at((double)value_of(key) - zmax);
+  }
+  __device__ __forceinline__ double weight_at(double x) const {
     if (!(x > -50.0)) return 0.0;  // below 2^-72
-    const double t = fma(x, 369.3299304675746, 6755399441055744.0);  // 256 / ln 2; 1.5 * 2^52 rounds to an integer
+    const double t = fma(x, 23.083120654223414, 6755399441055744.0);  // 16 / ln 2; 1.5 * 2^52 rounds to an integer
     const int k = __double2loint(t);
-    const double r = fma(t - 6755399441055744.0, -0.0027076061740622863, x);  // ln 2 / 256
-    double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+    const double r = fma(t - 6755399441055744.0, -0.04332169878499658, x);  // ln 2 / 16
+    double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
     const double w = p * s.table[k & (kTable - 1)];
-    return __hiloint2double(__double2hiint(w) + ((k >> 8) << 20), __double2loint(w));
+    return __hiloint2double(__double2hiint(w) + ((k >> 4) << 20), __double2loint(w));
   }
   // rounded to an integer; w < 2^51
-  __device__ __forceinline__ unsigned long long fixed(double w) const {
-    return (unsigned long long)(__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffll);
+  __device__ __forceinline__ u64 fixed(double w) const {
+    return (u64)(__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffll);
   }
 
-  // bins of the first pass: 1/32 wide below the maximum, the last one open
-  __device__ __forceinline__ int linear_bin(uint32_t key) const {
-    if (key == top_key) return 0;
-    return (int)fminf((zmax - value_of(key)) * 32.f, (float)(kBins - 1));
+  // bins of the first pass: bin b is within 1/64 of ref - b / 32; the first and the last (with NaN) are open
+  __device__ __forceinline__ int linear_bin(float z) const {
+    const float b = fmaxf(fminf((ref - z) * 32.f, (float)(kBins - 1)), 0.f);
+    return __float_as_int(b + 8388608.f) & (kBins - 1);  // 2^23 rounds to an integer
   }
 
-  // Adds the elements with lo <= key <= hi to this block's histogram.
-  template <bool MASS, typename Bin> __device__ __forceinline__ void count(uint32_t lo, uint32_t hi, Bin bin_of) {
-    Hist& h = s.hist[level & 1];
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-      h.n[i] = 0u;
-      if constexpr (MASS) h.m0[i] = h.m1[i] = h.m2[i] = 0u;
+  template <bool MASS> __device__ __forceinline__ void clear() {
+    s.n[threadIdx.x] = 0u;
+    if constexpr (MASS) s.m0[threadIdx.x] = s.m1[threadIdx.x] = s.m2[threadIdx.x] = 0u;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void add_mass(int b, u64 m) {
+    const uint32_t mask = (1u << a.limb) - 1u;
+    atomicAdd(&s.m0[b], (uint32_t)m & mask);
+    atomicAdd(&s.m1[b], (uint32_t)(m >> a.limb) & mask);
+    atomicAdd(&s.m2[b], (uint32_t)(m >> 2 * a.limb));
+  }
+  __device__ __forceinline__ u64 bin_mass(int b) const {
+    return (u64)s.m0[b] + ((u64)s.m1[b] << a.limb) + ((u64)s.m2[b] << 2 * a.limb);
+  }
+  // Adds the elements `in` to bins b; a warp whose elements share a bin (equal logits) adds once.
+  __device__ __forceinline__ void add(bool in, int b, u64 m) {
+    const unsigned active = __ballot_sync(0xffffffffu, in);
+    if (!active) return;
+    const int lead = __ffs(active) - 1;
+    const int lead_b = __shfl_sync(0xffffffffu, b, lead);  // by every lane, so not inside the ||
+    const bool same = __all_sync(0xffffffffu, !in || b == lead_b);
+    if (in) atomicAdd(&s.n[b], 1u);
+    if (same) {
+      if (!in) m = 0ull;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);  // < 2^52
+    }
+    if (same ? (threadIdx.x & 31) == lead : in) add_mass(b, m);
+  }
+
+  __device__ __forceinline__ u64 block_sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = s.scan[threadIdx.x & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    return v;
+  }
+  // sum of the threads in front, and of all
+  __device__ __forceinline__ u64 block_before(u64 v, u64& all) {
+    const u64 incl = warp_scan(v);
+    if ((threadIdx.x & 31) == 31) s.scan[threadIdx.x >> 5] = incl;
+    __syncthreads();
+    const u64 w = warp_scan(s.scan[threadIdx.x & 31]);
+    const int wid = threadIdx.x >> 5;
+    const u64 before = __shfl_sync(0xffffffffu, w, max(wid - 1, 0));
+    all = __shfl_sync(0xffffffffu, w, 31);
+    __syncthreads();
+    return (wid ? before : 0ull) + incl - v;
+  }
+
+  // The bin where base + the running count (MASS: weight) reaches (passes) `want`: s.bin, s.bin_n, s.ahead.
+  template <bool MASS> __device__ __forceinline__ void find(u64 base, u64 want) {
+    __syncthreads();
+    const int b = threadIdx.x;
+    const uint32_t c = s.n[b];
+    const u64 v = MASS ? bin_mass(b) : (u64)c;
+    u64 all;
+    const u64 run = base + block_before(v, all), next = run + v;
+    if (MASS ? (run <= want && next > want) : (run < want && next >= want)) {
+      s.bin = b;
+      s.bin_n = c;
+      s.ahead = run;
     }
     __syncthreads();
-    for (int i0_ = 0; i0_ < n; i0_ += kThreads) {
-      const int i = i0_ + threadIdx.x;
-      const uint32_t key = i < n ? key_at(i) : 0u;
-      const bool in = i < n && key >= lo && key <= hi;
-      const unsigned active = __ballot_sync(0xffffffffu, in);
-      if (!active) continue;
-      const int b = in ? bin_of(key) : 0;
-      // a warp whose elements share a bin (masked rows, equal logits) adds once
-      const int lead = __ffs(active) - 1;
-      const int b0 = __shfl_sync(0xffffffffu, b, lead);
-      const bool same = __all_sync(0xffffffffu, !in || b == b0);
-      unsigned long long m = 0ull;
-      if constexpr (MASS)
-        if (in) m = fixed(weight(key));
-      if (same) {
-        if constexpr (MASS) {
-          m = warp_sum64(m);  // < 2^52
-        }
-        if ((threadIdx.x & 31) == lead) {
-          atomicAdd(&h.n[b], __popc(active));
-          if constexpr (MASS) {
-            atomicAdd(&h.m0[b], (uint32_t)(m & 0xffffu));
-            atomicAdd(&h.m1[b], (uint32_t)(m >> 16 & 0xffffu));
-            atomicAdd(&h.m2[b], (uint32_t)(m >> 32));
-          }
-        }
-      } else if (in) {
-        atomicAdd(&h.n[b], 1u);
-        if constexpr (MASS) {
-          if (m & 0xffffu) atomicAdd(&h.m0[b], (uint32_t)(m & 0xffffu));
-          if (m >> 16 & 0xffffu) atomicAdd(&h.m1[b], (uint32_t)(m >> 16 & 0xffffu));
-          if (m >> 32) atomicAdd(&h.m2[b], (uint32_t)(m >> 32));
-        }
-      }
-    }
   }
 
-  // Sums the blocks' histograms and finds the bin where the running count (or
-  // weight) passes `want`: the first with base + running >= want (count), > want
-  // (weight).  Returns the sum over all bins.  `scale_p` >= 0: want becomes
-  // floor(scale_p * that sum) first.
-  template <bool MASS>
-  __device__ __forceinline__ unsigned long long find(unsigned long long base, unsigned long long& want, double scale_p) {
-    cluster_sync();
-    constexpr int PER = kBins / kThreads;
-    const Hist* h = &s.hist[level & 1];
-    unsigned long long v[PER];
-    uint32_t c[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      v[k] = 0ull;
-      c[k] = 0u;
-    }
-    for (int r = 0; r < blocks; ++r) {
-      const Hist* p = peer(h, r);
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const int b = threadIdx.x * PER + k;
-        c[k] += p->n[b];
-        if constexpr (MASS)
-          v[k] += (unsigned long long)p->m0[b] + ((unsigned long long)p->m1[b] << 16) +
-                  ((unsigned long long)p->m2[b] << 32);
-      }
-    }
-    unsigned long long mine = 0ull;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      if constexpr (!MASS) v[k] = c[k];
-      mine += v[k];
-    }
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    unsigned long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    if (lane == 31) s.scan[wid] = incl;
+  // From the counts of the first pass: the bins between which the running
+  // weight passes p times its sum.  The elements of bin b weigh between
+  // exp(ref - (b + 1/2) / 32 - zmax) and exp(ref - (b - 1/2) / 32 - zmax), with
+  // 1e-5 for the rounding of z - ref and 1 for that of a weight.
+  __device__ __forceinline__ void bracket(double p) {
     __syncthreads();
-    unsigned long long before = 0ull, total = 0ull;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < wid) before += s.scan[w];
-      total += s.scan[w];
+    const int b = threadIdx.x;
+    const uint32_t c = s.n[b];
+    const double top = (double)ref - zmax;
+    const double up = c * (fmin(b ? weight_at(top - (b - 0.5) * (1.0 / 32.0)) * (1.0 + 1e-5) : s.table[0], s.table[0]) + 1.0);
+    const double low =
+        b == kBins - 1 ? 0.0 : c * fmax(weight_at(top - (b + 0.5) * (1.0 / 32.0)) * (1.0 - 1e-5) - 1.0, 0.0);
+    if (b == 0) {
+      s.bin_lo = kBins - 1;
+      s.bin_hi = 0;
     }
-    if (scale_p >= 0.0) want = (unsigned long long)floor(scale_p * (double)total);
-    unsigned long long run = base + before + incl - mine;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const unsigned long long next = run + v[k];
-      if (MASS ? (run <= want && next > want) : (run < want && next >= want)) {
-        s.bin = threadIdx.x * PER + k;
-        s.bin_n = c[k];
-        s.ahead = run;
-      }
-      run = next;
+    const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const double iu = warp_scan(up), il = warp_scan(low);
+    if (lane == 31) {
+      s.scan_d[wid][0] = iu;
+      s.scan_d[wid][1] = il;
     }
     __syncthreads();
-    ++level;
-    return total;
+    const double su = warp_scan(s.scan_d[lane][0]), sl = warp_scan(s.scan_d[lane][1]);
+    const double all_u = __shfl_sync(0xffffffffu, su, 31), all_l = __shfl_sync(0xffffffffu, sl, 31);
+    const double bu = __shfl_sync(0xffffffffu, su, max(wid - 1, 0)), bl = __shfl_sync(0xffffffffu, sl, max(wid - 1, 0));
+    const double ru = (wid ? bu : 0.0) + iu, rl = (wid ? bl : 0.0) + il - low;
+    if (c && ru > p * all_l * (1.0 - 1e-12) - 1.0) atomicMin(&s.bin_lo, b);
+    if (c && rl <= p * all_u * (1.0 + 1e-12)) atomicMax(&s.bin_hi, b);
+    __syncthreads();
   }
 
-  // Key range of a bin of the first pass: its edges by bisection (linear_bin falls as the key grows).
-  __device__ __forceinline__ void edges(int bin, uint32_t& lo, uint32_t& hi) {
-    if (threadIdx.x < 64 && (threadIdx.x & 31) == 0) {
-      const bool upper = threadIdx.x >= 32;
-      // lower edge: the smallest key with linear_bin <= bin; upper: the smallest with linear_bin < bin, less one
-      uint32_t a_ = kLowest, b_ = top_key;  // linear_bin(top_key) = 0
-      const int limit = upper ? bin - 1 : bin;
-      if (limit < 0) {
-        a_ = top_key + 1u;
-      } else {
-        while (a_ < b_) {
-          const uint32_t mid = a_ + (b_ - a_) / 2;
-          if (linear_bin(mid) <= limit) b_ = mid; else a_ = mid + 1;
+  // Key range of bins b0 .. b1 of the first pass (linear_bin falls as the key
+  // grows): warp 0 finds the smallest key with linear_bin <= b1, warp 1 the
+  // smallest with linear_bin < b0, each in seven 32-way steps.
+  __device__ __forceinline__ void edges(int b0, int b1, uint32_t& lo, uint32_t& hi) {
+    const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (wid < 2) {
+      const int limit = wid ? b0 - 1 : b1;
+      uint32_t at;  // the smallest key with linear_bin <= limit, or top_key + 1
+      uint32_t a_ = kLowest, b_ = top_key + 1u;  // the answer lies in [a_, b_]
+      while (a_ < b_) {
+        const uint32_t step = ((b_ - a_) >> 5) + 1u;
+        const uint32_t probe = step * lane < b_ - a_ ? a_ + step * lane : b_;
+        const unsigned yes = __ballot_sync(0xffffffffu, probe >= b_ || linear_bin(value_of(probe)) <= limit);
+        // (the probe at b_ counts as found, so some lane has one unless all probes lie beneath it)
+        const int first = yes ? __ffs(yes) - 1 : 32;
+        const uint32_t found = __shfl_sync(0xffffffffu, probe, first & 31);
+        if (first == 0) {
+          b_ = a_;
+        } else {
+          if (first < 32) b_ = found;
+          a_ = min(a_ + step * (first - 1) + 1u, b_);
         }
       }
-      s.edge[upper] = upper ? a_ - 1u : a_;
+      at = a_;
+      if (lane == 0) s.edge[wid] = wid ? at - 1u : at;
     }
     __syncthreads();
     lo = s.edge[0];
@@ -294,223 +377,340 @@ struct Row {
     __syncthreads();
   }
 
-  // The key at which the running count reaches `want`, or the running weight
-  // passes it, among keys >= floor_key.  On return every key >= the result is
-  // in, except that of `ties_n` keys equal to it only a part may be (weight
-  // only; ahead = the weight of larger keys).
+  // Narrows [lo, hi] to the key at which the running count (MASS: weight) in
+  // front of which `ahead` lies reaches (passes) `want`.  Keys >= the result are
+  // in; MASS with ties_n > 1: of the ties_n keys equal to it only a part may be,
+  // `ahead` being the weight of larger keys.  `first`: ahead is not known yet.
   template <bool MASS>
-  __device__ __forceinline__ uint32_t select(uint32_t floor_key, unsigned long long want, double scale_p,
-                                             unsigned long long& ahead, uint32_t& ties_n, unsigned long long& target) {
-    count<MASS>(floor_key, top_key, [&](uint32_t k) { return linear_bin(k); });
-    find<MASS>(0ull, want, scale_p);
-    target = want;
-    uint32_t lo, hi;
-    int bin = s.bin;
-    uint32_t bn = s.bin_n;
-    ahead = s.ahead;
-    edges(bin, lo, hi);
-    lo = max(lo, floor_key);
+  __device__ __forceinline__ uint32_t narrow(uint32_t lo, uint32_t hi, u64 want, u64& ahead, uint32_t& ties_n,
+                                             bool first) {
+    ties_n = 0;
     while (true) {
-      ties_n = 0;
+      const int sh = max(0, 22 - __clz(hi - lo));  // (hi - lo) >> sh < 1024
+      clear<MASS>();
+      u64 sum = 0ull;
+      each([&](uint32_t key, int) {
+        const bool in = key >= lo && key <= hi;
+        const int b = in ? (int)((hi - key) >> sh) : 0;
+        if constexpr (MASS) {
+          if (first && key > hi) sum += fixed(weight(key));
+          add(in, b, in ? fixed(weight(key)) : 0ull);
+        } else {
+          if (in) atomicAdd(&s.n[b], 1u);
+        }
+      });
+      if (MASS && first) ahead = block_sum(sum);
+      first = false;
+      find<MASS>(ahead, want);
+      const uint32_t bn = s.bin_n, up = hi - ((uint32_t)s.bin << sh);
+      ahead = s.ahead;
+      const uint32_t width = (1u << sh) - 1u;
+      lo = up - lo > width ? up - width : lo;
+      hi = up;
       // the bin is in as a whole: one element (its weight crosses), or the count ends with it
       if (bn == 1u || (!MASS && ahead + bn == want)) return lo;
       if (lo == hi) {
         ties_n = bn;
         return lo;
       }
-      const int sh = max(0, 22 - __clz(hi - lo));  // (hi - lo) >> sh < 1024
-      const uint32_t hi0 = hi;
-      count<MASS>(lo, hi, [&](uint32_t k) { return (int)((hi0 - k) >> sh); });
-      unsigned long long w = want;
-      find<MASS>(ahead, w, -1.0);
-      bin = s.bin;
-      bn = s.bin_n;
-      ahead = s.ahead;
-      const uint32_t up = hi0 - ((uint32_t)bin << sh);
-      lo = max(lo, up - ((1u << sh) - 1u) > up ? 0u : up - ((1u << sh) - 1u));
-      hi = up;
+      __syncthreads();  // s.bin is read before the next search writes it
     }
   }
 };
 
-template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
-  const int blocks = (int)cg::this_cluster().num_blocks();
-  const int rank = (int)cg::this_cluster().block_rank();
+  constexpr int VEC = Row<T>::VEC;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  Shared& first = *cluster.map_shared_rank(&s, 0);
   uint32_t* seen_bits = reinterpret_cast<uint32_t*>(smem + sizeof(Shared));
-  uint32_t* keys = seen_bits + (a.seen ? (a.slice + 31) / 32 : 0);
-  const float temp = a.temp.at(row);
+  const int seen_words = a.seen ? ((a.V + 31) / 32 + 3) / 4 * 4 : 0;
+  uint2* list = reinterpret_cast<uint2*>(seen_bits + seen_words);
+  uint2* first_list = cluster.map_shared_rank(list, 0);
+  // all settings at once: each is a memory latency of its own
+  const float temp = a.temp.at(row), pen = a.penalty.at(row), min_p = fminf(a.min_p.at(row), 1.f);
+  const double p = (double)a.top_p.at(row), u = (double)a.u[row];
+  const int64_t want_k = a.top_k ? a.top_k[row] : a.top_k0;
   const bool greedy = !(temp > 0.f);
-  Row<T, RESIDENT> R{a, s, keys, seen_bits, (const T*)a.logits + row * a.ls, greedy ? 1.f : temp,
-                     a.penalty.at(row), row, rank, blocks, min(rank * a.slice, a.V), 0, 0u, 0.f, 0.0};
-  R.n = min(a.slice, a.V - R.i0);
-  for (int j = tid; j < kTable; j += kThreads) s.table[j] = ldexp(exp2((double)j / kTable), a.fbits);
-  if (a.seen) {
-    for (int i = tid; i < (a.slice + 31) / 32; i += kThreads) seen_bits[i] = 0u;
-    __syncthreads();
-    for (int i = tid; i < a.L; i += kThreads) {
-      const int64_t t = a.seen[row * a.seen_s + i] - R.i0;
-      if (t >= 0 && t < R.n) atomicOr(&seen_bits[t >> 5], 1u << (t & 31));
-    }
-    __syncthreads();
-  }
-  // keys into shared memory; the largest, and of its ties the first
-  uint32_t best = 0u;
-  int best_i = 0;
-  auto take = [&](float logit, int i) {
-    const uint32_t k = R.make_key(logit, i);
-    if constexpr (RESIDENT) keys[i] = k;
-    if (k > best) {  // a thread's indices grow
-      best = k;
-      best_i = R.i0 + i;
-    }
-  };
-  constexpr int VEC = Vec16<T>::N;
-  const T* src = R.lr + R.i0;
-  int done = 0;
-  if (((uintptr_t)src & 15) == 0) {
-    const int vecs = R.n / VEC;
-#pragma unroll 2
-    for (int v = tid; v < vecs; v += kThreads) {
-      float x[VEC];
-      load16<T>(src + v * VEC, x);
+  const T* lr = (const T*)a.logits + row * a.ls;
+  Row<T> R{a, s, seen_bits, list, lr, greedy ? 1.f : temp, pen, ((uintptr_t)lr & 7) == 0,
+           (greedy || temp == 1.f) && (a.seen == nullptr || pen == 1.f)};
+  // a first guess of the maximum, from the first vectors of the row
+  float guess = -INFINITY;
+  if (tid * VEC + VEC <= a.V)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) take(x[k], v * VEC + k);
-    }
-    done = vecs * VEC;
+    for (int k = 0; k < VEC; ++k) guess = fmaxf(guess, to_f<T>(lr[tid * VEC + k]));
+  if (tid < kTable) s.table[tid] = ldexp(exp2((double)tid / kTable), a.fbits);
+  s.n[tid] = s.m0[tid] = s.m1[tid] = s.m2[tid] = 0u;
+  if (tid == 0) {
+    s.list_n = s.bin = 0;
   }
-  for (int i = done + tid; i < R.n; i += kThreads) take(to_f<T>(src[i]), i);
-  unsigned long long packed = R.n > 0 ? ((unsigned long long)best << 32) | (0xffffffffu - (uint32_t)best_i) : 0ull;
+  if (!R.plain)
+    for (int i = tid; i < seen_words; i += kThreads) seen_bits[i] = 0u;
+  guess = warp_max(guess);
+  if (lane == 0) s.scan_f[wid] = guess;
+  __syncthreads();
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");  // the first block's counters are 0
+  if (a.seen && !R.plain) {
+    for (int i = tid; i < a.L; i += kThreads) {
+      const int64_t t = a.seen[row * a.seen_s + i];
+      if (t >= 0 && t < a.V) atomicOr(&seen_bits[t >> 5], 1u << (t & 31));
+    }
+    __syncthreads();
+  }
+  guess = warp_max(s.scan_f[lane]) / R.div;
+  R.ref = (isfinite(guess) ? guess : 0.f) + 4.f;
+  // first pass over this block's part: the largest (and for greedy rows, of its ties the first), and the counts
+  const int i0 = min(rank * a.slice, a.V), i1 = min(i0 + a.slice, a.V);
+  const bool by_count = want_k > 0 && want_k < a.V, by_mass = p < 1.0;
+  const bool filtered = by_count || by_mass || min_p > 0.f;
+  u64 packed = 0ull;
+  if (greedy) {
+    R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (k < n) packed = max(packed, ((u64)R.key_or_low(z[k]) << 32) | (0xffffffffu - (uint32_t)(i + k)));
+    });
+  } else {
+    float zm = -INFINITY;
+    R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
+      if (n == VEC) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          zm = fmaxf(zm, z[k]);
+          if (filtered) atomicAdd(&s.n[R.linear_bin(z[k])], 1u);
+        }
+      } else if (n) {
+        zm = fmaxf(zm, z[0]);
+        if (filtered) atomicAdd(&s.n[R.linear_bin(z[0])], 1u);
+      }
+    });
+    packed = (u64)key_of(zm) << 32;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) packed = max(packed, __shfl_xor_sync(0xffffffffu, packed, o));
   if (lane == 0) s.scan[wid] = packed;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) packed = max(packed, s.scan[w]);
-    s.best = packed;
+  if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+  if (wid == 0) {
+    packed = s.scan[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) packed = max(packed, __shfl_xor_sync(0xffffffffu, packed, o));
+    if (lane == 0) first.best[rank] = packed;
   }
-  R.cluster_sync();
-  for (int r = 0; r < blocks; ++r) packed = max(packed, *R.peer(&s.best, r));
-  R.top_key = (uint32_t)(packed >> 32);
-  R.zmax = value_of(R.top_key);
-  R.zmax_d = (double)R.zmax;
-  const int top_i = (int)(0xffffffffu - (uint32_t)packed);
-  if (greedy || R.top_key <= kLowest) {
-    if (rank == 0 && tid == 0) {
-      a.token[row] = top_i;
-      a.logprob[row] = greedy ? 0.f : __int_as_float(0x7fffffff);
+  if (rank > 0 && filtered && s.n[tid]) atomicAdd(&first.n[tid], s.n[tid]);
+  R.cluster_sync(blocks);
+  // the first block decides which keys may still be kept: [lo, top_key]; of them [lo, hi] hold the border
+  uint32_t lo = kLowest, hi = 0u, threshold = kLowest, ties_n = 0;
+  u64 ahead = 0ull, want = 0ull;
+  bool open = false;  // the k-th largest lies strictly inside [lo, hi]
+  if (rank == 0) {
+    u64 best = s.best[0];
+    for (int r = 1; r < blocks; ++r) best = max(best, s.best[r]);
+    R.set_top((uint32_t)(best >> 32));
+    hi = R.top_key;
+    const bool done = greedy || R.top_key <= kLowest;
+    bool fits = false;
+    if (done) {
+      if (tid == 0) {
+        a.token[row] = greedy ? (int64_t)(0xffffffffu - (uint32_t)best) : 0;
+        a.logprob[row] = greedy ? 0.f : __int_as_float(0x7fffffff);
+      }
+    } else if (filtered) {
+      if (by_count) {
+        want = (u64)want_k;
+        R.template find<false>(0ull, want);
+        ahead = s.ahead;
+        open = !(s.bin_n == 1u || ahead + s.bin_n == want);
+        R.edges(s.bin, s.bin, lo, hi);
+      } else if (by_mass) {
+        R.bracket(fmax(p, 0.0));
+        R.edges(s.bin_lo, max(s.bin_lo, s.bin_hi), lo, hi);
+      }
+      if (min_p > 0.f && !by_count) {
+        // exp(z - zmax) >= min_p, with room for the logarithm's rounding and that of the sum
+        const float zmax = value_of(R.top_key);
+        const uint32_t least = key_of(zmax + (logf(min_p) - 1e-3f) - fabsf(zmax) * 1e-6f);
+        lo = max(lo, min(least, R.top_key));
+        hi = max(hi, lo);
+      }
+      const int last = R.linear_bin(value_of(lo));
+      fits = R.block_sum(tid <= last ? s.n[tid] : 0u) <= (u64)a.list_cap;
     }
-    R.cluster_sync();  // the peers may still read this block's maximum
+    if (tid == 0) {
+      s.top_key = R.top_key;
+      s.lo = lo;
+      s.done = done;
+      s.listing = fits;
+      s.summing = by_mass && !by_count;
+    }
+  }
+  R.cluster_sync(blocks);
+  if (first.done) {
+    R.cluster_sync(blocks);  // nobody leaves while `first` is read
     return;
   }
-  unsigned long long ahead = 0ull, target = 0ull;
-  uint32_t threshold = kLowest, ties_n = 0;
-  const int64_t want = a.top_k ? a.top_k[row] : a.top_k0;
-  if (want > 0 && want < a.V)
-    threshold = R.template select<false>(kLowest, (unsigned long long)want, -1.0, ahead, ties_n, target);
-  // how many keys equal to the threshold are in
-  unsigned long long ties_in = ~0ull;
-  const double p = (double)a.top_p.at(row);
-  if (p < 1.0) {
-    threshold = R.template select<true>(threshold, 0ull, fmax(p, 0.0), ahead, ties_n, target);
-    if (ties_n > 1) {
-      const unsigned long long w = R.fixed(R.weight(threshold));
-      ties_in = (target - ahead) / w + 1ull;  // w > 0: the running weight crosses within these ties
-      if (ties_in >= ties_n) ties_in = ~0ull;
-    }
+  const bool listing = first.listing, summing = first.summing;
+  if (rank > 0) {
+    R.set_top(first.top_key);
+    lo = first.lo;
   }
-  const double least = (double)a.min_p.at(row) * s.table[0];
-  // each warp a contiguous run of the slice, so that running sums follow the index
-  const int per = ((R.n + kWarps - 1) / kWarps + 31) & ~31;
-  const int w0 = min(wid * per, R.n), w1 = min(w0 + per, R.n);
-  unsigned long long tie_base = 0ull;
-  if (ties_in != ~0ull) {  // the same in every block of the row
-    uint32_t t = 0;
-    for (int i = w0; i < w1; i += 32) t += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && R.key_at(i + lane) == threshold));
-    if (lane == 0) s.warp_ties[wid] = t;
+  const int ish = a.index_shift;
+  const double least = (double)min_p * s.table[0];
+  // second pass: the list of keys >= lo and the sum of all weights; without a filter, the weight of each index bin
+  if (!filtered) {
+    R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
+      u64 m = 0ull;
+      int b = i >> ish;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (k < n) {
+          if ((i + k) >> ish != b) {  // bins shorter than a vector
+            if (m) R.add_mass(b, m);
+            m = 0ull;
+            b = (i + k) >> ish;
+          }
+          m += R.fixed(R.weight(R.key_or_low(z[k])));
+        }
+      if (m) R.add_mass(b, m);
+    });
     __syncthreads();
-    if (tid == 0) {
-      uint32_t all = 0;
-      for (int w = 0; w < kWarps; ++w) all += s.warp_ties[w];
-      s.ties = all;
+    if (rank > 0) {  // the bins of a block's part are its own
+      const int b = (i0 >> ish) + tid;
+      if (i0 < i1 && b <= (i1 - 1) >> ish) {
+        first.m0[b] = s.m0[b];
+        first.m1[b] = s.m1[b];
+        first.m2[b] = s.m2[b];
+      }
     }
-    R.cluster_sync();
-    for (int r = 0; r < rank; ++r) tie_base += *R.peer(&s.ties, r);
-    for (int w = 0; w < wid; ++w) tie_base += s.warp_ties[w];
+  } else if (listing || summing) {
+    const float lo_z = value_of(lo);
+    const bool all_in = lo <= kLowest;
+    u64 sum = 0ull;
+    R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
+      if (summing) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (k < n) sum += R.fixed(R.weight(R.key_or_low(z[k])));
+      }
+      if (listing) {
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) c += k < n && (z[k] >= lo_z || all_in);
+        if (__any_sync(0xffffffffu, c > 0)) {
+          const int incl = warp_scan(c);
+          int at = 0;
+          if (lane == 31) at = atomicAdd(&first.list_n, incl);
+          at = __shfl_sync(0xffffffffu, at, 31) + incl - c;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            if (k < n && (z[k] >= lo_z || all_in)) first_list[at++] = make_uint2(R.key_or_low(z[k]), (uint32_t)(i + k));
+        }
+      }
+    });
+    if (summing) {
+      sum = R.block_sum(sum);
+      if (tid == 0) first.total[rank] = sum;
+    }
   }
-  // kept weight of element i + lane; `tie` counts the threshold's ties in front of this step
-  auto kept = [&](int i, unsigned long long& tie) -> unsigned long long {
-    const uint32_t key = i + lane < w1 ? R.key_at(i + lane) : 0u;
-    bool in = key >= threshold && i + lane < w1;
-    if (ties_in != ~0ull) {
-      const unsigned eq = __ballot_sync(0xffffffffu, in && key == threshold);
-      if (key == threshold && tie + __popc(eq & ((1u << lane) - 1u)) >= ties_in) in = false;
-      tie += __popc(eq);
+  R.cluster_sync(blocks);
+  if (rank > 0) return;  // the rest is the first block's alone
+  u64 total = 0ull;
+  if (by_mass && !by_count)
+    for (int r = 0; r < blocks; ++r) total += s.total[r];
+  R.listed = listing;
+  if (by_count) threshold = open ? R.template narrow<false>(lo, hi, want, ahead, ties_n, false) : lo;
+  u64 ties_in = ~0ull;  // how many keys equal to the threshold are in
+  if (by_mass) {
+    const bool whole = hi == R.top_key;  // nothing lies in front of [lo, hi]
+    if (by_count) {
+      lo = threshold;
+      hi = R.top_key;
     }
-    if (!in) return 0ull;
+    u64 inside = 0ull;
+    if (by_count || min_p > 0.f) {
+      R.each([&](uint32_t key, int) {
+        if (key >= lo) inside += R.fixed(R.weight(key));
+      });
+      inside = R.block_sum(inside);
+    }
+    if (by_count) total = inside;
+    want = (u64)floor(fmax(p, 0.0) * (double)total);
+    ahead = 0ull;
+    if (!by_count && min_p > 0.f && inside <= want) {
+      threshold = lo;  // min-p cuts in front of the nucleus' border
+    } else {
+      threshold = R.template narrow<true>(lo, hi, want, ahead, ties_n, !by_count && !whole);
+      if (ties_n > 1) {
+        ties_in = (want - ahead) / R.fixed(R.weight(threshold)) + 1ull;  // weight > 0: the sum crosses within these ties
+        if (ties_in >= ties_n) ties_in = ~0ull;
+      }
+    }
+  }
+  // of the threshold's ties those up to this index
+  int tie_last = a.V;
+  if (ties_in != ~0ull) {
+    __syncthreads();
+    R.template clear<false>();
+    R.each([&](uint32_t key, int i) {
+      if (key == threshold) atomicAdd(&s.n[i >> ish], 1u);
+    });
+    R.template find<false>(0ull, ties_in);
+    const int i = (s.bin << ish) + tid;
+    const bool tie = tid < (1 << ish) && i < a.V && R.key_at(i) == threshold;
+    const u64 base = s.ahead;
+    u64 all;
+    const u64 before = base + R.block_before(tie ? 1ull : 0ull, all);
+    if (tie && before + 1ull == ties_in) s.at = i;
+    __syncthreads();
+    tie_last = s.at;
+  }
+  auto kept = [&](uint32_t key, int i) -> u64 {
+    if (key < threshold || key == 0u || (key == threshold && i > tie_last)) return 0ull;
     const double w = R.weight(key);
     return w >= least ? R.fixed(w) : 0ull;
   };
-  unsigned long long mine = 0ull, tie = tie_base;
-  for (int i = w0; i < w1; i += 32) mine += kept(i, tie);
-  mine = warp_sum64(mine);
-  if (lane == 0) s.warp_mass[wid] = mine;
-  __syncthreads();
-  if (tid == 0) {
-    unsigned long long all = 0ull;
-    for (int w = 0; w < kWarps; ++w) all += s.warp_mass[w];
-    s.mass = all;
+  // the draw: kept weight by index
+  if (filtered) {
+    __syncthreads();
+    R.template clear<true>();
+    R.each([&](uint32_t key, int i) {
+      const u64 m = kept(key, i);
+      if (m) R.add_mass(i >> ish, m);
+    });
+    __syncthreads();
   }
-  R.cluster_sync();
-  unsigned long long total = 0ull, base = 0ull;
-  for (int r = 0; r < blocks; ++r) {
-    const unsigned long long m = *R.peer(&s.mass, r);
-    if (r < rank) base += m;
-    total += m;
-  }
-  for (int w = 0; w < wid; ++w) base += s.warp_mass[w];
+  u64 sum = R.bin_mass(tid), all;
+  const u64 run = R.block_before(sum, all);
   // run > u * total for the integer run means run > floor(u * total); u = 1 ends at the last kept token
-  unsigned long long goal = (unsigned long long)floor(fmax((double)a.u[row], 0.0) * (double)total);
-  goal = min(goal, total - 1ull);
-  if (base <= goal && goal < base + mine) {  // one warp of the row
-    tie = tie_base;
-    for (int i = w0; i < w1; i += 32) {
-      const unsigned long long m = kept(i, tie);
-      unsigned long long incl = m;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, base + incl > goal);
-      if (over) {
-        if (lane == __ffs(over) - 1) {
-          a.token[row] = R.i0 + i + lane;
-          const float z = value_of(R.key_at(i + lane));
-          const double x = R.key_at(i + lane) == R.top_key ? 0.0 : (double)z - R.zmax_d;
-          a.logprob[row] = (float)(x - log((double)total / s.table[0]));
-        }
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, incl, 31);
+  const u64 goal = min((u64)floor(fmax(u, 0.0) * (double)all), all - 1ull);
+  if (run <= goal && run + sum > goal) {
+    s.bin = tid;
+    s.ahead = run;
+  }
+  __syncthreads();
+  {
+    const int i = (s.bin << ish) + tid;
+    const bool on = tid < (1 << ish) && i < a.V;
+    const uint32_t key = on ? R.key_at(i) : 0u;
+    const u64 m = kept(key, i);
+    u64 ignored;
+    const u64 base = s.ahead;
+    const u64 in_front = base + R.block_before(m, ignored);
+    if (on && in_front <= goal && in_front + m > goal) {
+      a.token[row] = i;
+      a.logprob[row] = (float)((key == R.top_key ? 0.0 : (double)value_of(key) - R.zmax) - log((double)all / s.table[0]));
     }
   }
-  R.cluster_sync();  // the peers may still read this block's sums
 }
 
-template <typename T, bool RESIDENT>
+template <typename T>
 void launch_sample(const SampleArgs& a, int64_t B, int cluster, size_t smem) {
-  static bool set[64] = {};
-  int dev = 0;
-  C10_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev >= 64 || !set[dev]) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T, RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(sizeof(Shared) + kMaxSlice * 4 + kMaxSlice / 8)));
-    if (dev < 64) set[dev] = true;
-  }
+  C10_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(B * cluster));
   cfg.blockDim = dim3(kThreads);
@@ -523,7 +723,7 @@ void launch_sample(const SampleArgs& a, int64_t B, int cluster, size_t smem) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sample_kernel<T, RESIDENT>, a));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
 }
 
 }  // namespace
@@ -582,24 +782,21 @@ std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const at::Tensor
     a.seen_s = seen->stride(0);
     a.L = (int)seen->size(1);
   }
-  // as many blocks a row as the GPU holds at once (two an SM), at least enough for the row to fit their memory
-  int cluster = 1;
-  while (cluster < kMaxCluster && (B * cluster * 2 <= 2 * num_sms() || (V + cluster - 1) / cluster > kMaxSlice) &&
-         V / (cluster * 2) >= 512)
-    cluster *= 2;
-  a.slice = (int)(((V + cluster - 1) / cluster + 31) / 32 * 32);
-  TORCH_CHECK(B * cluster < (1ll << 31), what, ": too many rows in one call");
+  TORCH_CHECK(B < (1ll << 28), what, ": too many rows in one call");
   int bits = 15;
   while ((1ll << bits) < V) ++bits;
-  a.fbits = 62 - bits;
-  const bool resident = a.slice <= kMaxSlice;
-  const size_t smem = sizeof(Shared) + (a.seen ? (a.slice + 31) / 32 * 4 : 0) + (resident ? (size_t)a.slice * 4 : 0);
-  TB_DISPATCH_FLOAT(logits.scalar_type(), what, [&] {
-    if (resident)
-      launch_sample<scalar_t, true>(a, B, cluster, smem);
-    else
-      launch_sample<scalar_t, false>(a, B, cluster, smem);
-  });
+  a.limb = std::min(16, 32 - bits);  // V limbs of this width sum to less than 2^32
+  a.fbits = std::min(62 - bits, 3 * a.limb - 1);
+  while ((V - 1) >> a.index_shift >= kBins) ++a.index_shift;
+  // blocks that help with the two passes over a row, while SMs are free and a part is worth their barriers
+  int cluster = 1;
+  while (cluster < 8 && B * cluster * 2 <= num_sms() && V / (cluster * 2) >= 2048) cluster *= 2;
+  a.slice = (int)((V + cluster - 1) / cluster);
+  if (cluster > 1) a.slice = (((a.slice - 1) >> a.index_shift) + 1) << a.index_shift;  // whole index bins, of 4 or more
+  const size_t fixed = sizeof(Shared) + (a.seen ? ((V + 31) / 32 + 3) / 4 * 16 : 0);
+  a.list_cap = (int)std::min<int64_t>(V, (int64_t)(kSharedLimit - fixed) / 8);
+  const size_t smem = fixed + (size_t)a.list_cap * 8;
+  TB_DISPATCH_FLOAT(logits.scalar_type(), what, [&] { launch_sample<scalar_t>(a, B, cluster, smem); });
   check_launch(what);
   return {token, logprob};
 }

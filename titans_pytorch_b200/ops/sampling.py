@@ -58,7 +58,7 @@ def sample_tokens_reference(logits, uniform, temperature, top_k, top_p, min_p, g
     ahead = torch.cumsum(ranked, dim=1) - ranked
     nucleus = torch.where(top_p >= 1, torch.full_like(ranked[:, 0], float("inf")), top_p.double() * ranked.sum(dim=1))
     keep = torch.zeros_like(w, dtype=torch.bool).scatter_(1, order, ahead <= nucleus.clamp(min=0)[:, None])
-    w = torch.where(keep & (w >= min_p.double()[:, None]), w, torch.zeros_like(w))
+    w = torch.where(keep & (w >= min_p.double().clamp(max=1)[:, None]), w, torch.zeros_like(w))
     reach = torch.cumsum(w, dim=1)
     token = (reach <= uniform.double()[:, None] * reach[:, -1:]).sum(dim=1)
     last = torch.where(w > 0, torch.arange(V, device=z.device), -1).amax(dim=1)
