@@ -17,25 +17,30 @@
 // fit; the borders of running sums are off by the square root of V such
 // roundings at most, where fp32 sums would move tokens.
 //
-// Nothing is sorted.  The first pass over the row takes the maximum and counts
-// elements in 1024 bins linear in z (1/32 wide, around a sampled maximum).  From
-// the counts follow the bin of the k-th largest, or, for top-p, two bins between
-// which the border must lie (a bin's elements weigh the same within 3 %).  The
-// second pass (the row is in L2 now) sums the exact weights and moves every
-// element that may still be kept into a list in shared memory; if they do not
-// fit, later passes go on reading the row.  The list is narrowed by histograms
-// over the keys (order-preserving 32-bit images of z) until a bin decides: one
-// element, or one value.  The draw is the same search over the index: 1024
-// index bins, then the elements of one bin.
+// Nothing is sorted; a row is passed over two to four times (from L2 after the
+// first):
+//   1. the maximum (greedy rows: and its index; they are done);
+//   2. counts in 1024 bins linear in z, 1/32 wide below the maximum, and for
+//      top-p the exact sum of all weights;
+//   3. from the counts follow the bin of the k-th largest, or, as a bin's
+//      elements weigh the same within 3 %, two bins between which top-p's border
+//      must lie: their elements go to a list in shared memory, which is narrowed
+//      by histograms over the keys (order-preserving 32-bit images of z) until a
+//      bin decides: one element, or one value.  If they do not fit, the row is
+//      passed over instead;
+//   4. the draw is the same search over the index: kept weight in 1024 index
+//      bins, then the elements of one bin.
+// Rows without top-k and top-p need 1 and 4 only, and so do rows where min-p
+// cuts above top-p's border for certain; after 3 the draw works on the list if
+// that holds everything that may be kept.
 //
 // One block does all of this for a row; while SMs are free, up to seven more
-// take parts of the two passes and add their counts, sums and list entries to
-// its shared memory, three barriers in all.  (Every block of the cluster summing
-// all blocks' bins itself cost 2.5 us a search, and sorting nothing but keeping
-// the row in shared memory gained nothing over reading it again from L2.)
-// What bounds it: one row, the chain of block barriers; many rows of large
-// vocabularies, the instructions of the two passes (about 25 of the fp64
-// exponential and 25 of loads, keys and bins per element).
+// take parts of the passes and add their counts, sums and list entries to its
+// shared memory.  (Letting every block of a cluster sum all blocks' bins itself
+// cost 2.5 us a search, and keeping the row in shared memory gained nothing.)
+// What bounds it: one row, the chain of barriers (a cluster's costs about 1 us
+// with the read behind it); many rows, the instructions of the passes: 5 to 12
+// an element, 45 more where its fp64 exponential is wanted.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -89,16 +94,18 @@ struct __align__(16) Shared {
   uint32_t n[kBins], m0[kBins], m1[kBins], m2[kBins];  // count; weight in three limbs (shared memory adds 32 bits)
   u64 scan[kWarps];
   double scan_d[kWarps][2];
-  float scan_f[kWarps];
   int bin, bin_lo, bin_hi, at;
   uint32_t bin_n;
   u64 ahead;
   uint32_t edge[2];
   // of the row's first block: what the others add to, and what it tells them
   u64 best[8], total[8];  // by block (64-bit atomics on another block's shared memory lost updates)
-  uint32_t top_key, lo;
-  int list_n, done, listing, summing;
+  uint32_t lo, hi, threshold;
+  int list_n, route, tie_last;
 };
+
+// what the first block makes the others do after the counts
+enum Route : int { DRAW = 0, LIST_ALL = 1, LIST_BORDER = 2, ALONE = 3 };
 
 template <typename V> __device__ __forceinline__ V warp_scan(V v) {  // inclusive
   const int lane = threadIdx.x & 31;
@@ -122,13 +129,14 @@ struct Row {
   bool vec;           // 8-byte loads
   bool plain;         // z is the logit
   bool listed = false;
-  float ref = 0.f;    // upper edge of bin 0 of the first pass
+  float zmax_f = 0.f;
   uint32_t top_key = 0u;
   double zmax = 0.0;
 
   __device__ __forceinline__ void set_top(uint32_t key) {
     top_key = key;
-    zmax = (double)value_of(key);
+    zmax_f = value_of(key);
+    zmax = (double)zmax_f;
   }
   static __device__ __forceinline__ void cluster_sync(int blocks) {
     if (blocks > 1)
@@ -237,9 +245,10 @@ struct Row {
     return (u64)(__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffll);
   }
 
-  // bins of the first pass: bin b is within 1/64 of ref - b / 32; the first and the last (with NaN) are open
+  // bins of the counts: bin b is within 1/64 of zmax - b / 32; the last (with NaN) is open
   __device__ __forceinline__ int linear_bin(float z) const {
-    const float b = fmaxf(fminf((ref - z) * 32.f, (float)(kBins - 1)), 0.f);
+    const float d = z == zmax_f ? 0.f : zmax_f - z;  // (both may be infinite)
+    const float b = fminf(d * 32.f, (float)(kBins - 1));
     return __float_as_int(b + 8388608.f) & (kBins - 1);  // 2^23 rounds to an integer
   }
 
@@ -313,21 +322,20 @@ struct Row {
     __syncthreads();
   }
 
-  // From the counts of the first pass: the bins between which the running
-  // weight passes p times its sum.  The elements of bin b weigh between
-  // exp(ref - (b + 1/2) / 32 - zmax) and exp(ref - (b - 1/2) / 32 - zmax), with
-  // 1e-5 for the rounding of z - ref and 1 for that of a weight.
-  __device__ __forceinline__ void bracket(double p) {
+  // From the counts: the bins between which the running weight passes `want`
+  // (s.bin_lo, s.bin_hi).  The elements of bin b weigh between
+  // exp(-(b + 1/2) / 32) and exp(-(b - 1/2) / 32), with 1e-5 for the rounding of
+  // z - zmax and 1 for that of a weight.  `want` < 0: p times the least that all
+  // weigh; then s.bin tells whether bins 0 .. last weigh no more than that for certain.
+  __device__ __forceinline__ void bracket(double want, double p, int last) {
     __syncthreads();
     const int b = threadIdx.x;
     const uint32_t c = s.n[b];
-    const double top = (double)ref - zmax;
-    const double up = c * (fmin(b ? weight_at(top - (b - 0.5) * (1.0 / 32.0)) * (1.0 + 1e-5) : s.table[0], s.table[0]) + 1.0);
-    const double low =
-        b == kBins - 1 ? 0.0 : c * fmax(weight_at(top - (b + 0.5) * (1.0 / 32.0)) * (1.0 - 1e-5) - 1.0, 0.0);
+    const double up = c * (fmin(weight_at((0.5 - b) * (1.0 / 32.0)) * (1.0 + 1e-5), s.table[0]) + 1.0);
+    const double low = b == kBins - 1 ? 0.0 : c * fmax(weight_at((-0.5 - b) * (1.0 / 32.0)) * (1.0 - 1e-5) - 1.0, 0.0);
     if (b == 0) {
       s.bin_lo = kBins - 1;
-      s.bin_hi = 0;
+      s.bin_hi = s.bin = 0;
     }
     const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const double iu = warp_scan(up), il = warp_scan(low);
@@ -337,15 +345,19 @@ struct Row {
     }
     __syncthreads();
     const double su = warp_scan(s.scan_d[lane][0]), sl = warp_scan(s.scan_d[lane][1]);
-    const double all_u = __shfl_sync(0xffffffffu, su, 31), all_l = __shfl_sync(0xffffffffu, sl, 31);
+    const double all_l = __shfl_sync(0xffffffffu, sl, 31);
     const double bu = __shfl_sync(0xffffffffu, su, max(wid - 1, 0)), bl = __shfl_sync(0xffffffffu, sl, max(wid - 1, 0));
     const double ru = (wid ? bu : 0.0) + iu, rl = (wid ? bl : 0.0) + il - low;
-    if (c && ru > p * all_l * (1.0 - 1e-12) - 1.0) atomicMin(&s.bin_lo, b);
-    if (c && rl <= p * all_u * (1.0 + 1e-12)) atomicMax(&s.bin_hi, b);
+    if (want < 0.0) {
+      if (b == last) s.bin = ru * (1.0 + 1e-9) + 1.0 < p * all_l;
+    } else {
+      if (c && ru > want * (1.0 - 1e-12) - 1.0) atomicMin(&s.bin_lo, b);
+      if (c && rl <= want * (1.0 + 1e-12)) atomicMax(&s.bin_hi, b);
+    }
     __syncthreads();
   }
 
-  // Key range of bins b0 .. b1 of the first pass (linear_bin falls as the key
+  // Key range of bins b0 .. b1 of the counts (linear_bin falls as the key
   // grows): warp 0 finds the smallest key with linear_bin <= b1, warp 1 the
   // smallest with linear_bin < b0, each in seven 32-way steps.
   __device__ __forceinline__ void edges(int b0, int b1, uint32_t& lo, uint32_t& hi) {
@@ -439,37 +451,23 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   const T* lr = (const T*)a.logits + row * a.ls;
   Row<T> R{a, s, seen_bits, list, lr, greedy ? 1.f : temp, pen, ((uintptr_t)lr & 7) == 0,
            (greedy || temp == 1.f) && (a.seen == nullptr || pen == 1.f)};
-  // a first guess of the maximum, from the first vectors of the row
-  float guess = -INFINITY;
-  if (tid * VEC + VEC <= a.V)
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) guess = fmaxf(guess, to_f<T>(lr[tid * VEC + k]));
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
   if (tid < kTable) s.table[tid] = ldexp(exp2((double)tid / kTable), a.fbits);
   s.n[tid] = s.m0[tid] = s.m1[tid] = s.m2[tid] = 0u;
-  if (tid == 0) {
-    s.list_n = s.bin = 0;
-  }
-  if (!R.plain)
-    for (int i = tid; i < seen_words; i += kThreads) seen_bits[i] = 0u;
-  guess = warp_max(guess);
-  if (lane == 0) s.scan_f[wid] = guess;
-  __syncthreads();
-  if (blocks > 1) asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");  // the first block's counters are 0
+  if (tid == 0) s.list_n = s.bin = 0;
   if (a.seen && !R.plain) {
+    for (int i = tid; i < seen_words; i += kThreads) seen_bits[i] = 0u;
+    __syncthreads();
     for (int i = tid; i < a.L; i += kThreads) {
       const int64_t t = a.seen[row * a.seen_s + i];
       if (t >= 0 && t < a.V) atomicOr(&seen_bits[t >> 5], 1u << (t & 31));
     }
     __syncthreads();
   }
-  guess = warp_max(s.scan_f[lane]) / R.div;
-  R.ref = (isfinite(guess) ? guess : 0.f) + 4.f;
-  // first pass over this block's part: the largest (and for greedy rows, of its ties the first), and the counts
+  // 1. the largest of this block's part, and of the row
   const int i0 = min(rank * a.slice, a.V), i1 = min(i0 + a.slice, a.V);
-  const bool by_count = want_k > 0 && want_k < a.V, by_mass = p < 1.0;
-  const bool filtered = by_count || by_mass || min_p > 0.f;
   u64 packed = 0ull;
-  if (greedy) {
+  if (greedy) {  // of its ties the first
     R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
@@ -480,13 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
       if (n == VEC) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          zm = fmaxf(zm, z[k]);
-          if (filtered) atomicAdd(&s.n[R.linear_bin(z[k])], 1u);
-        }
+        for (int k = 0; k < VEC; ++k) zm = fmaxf(zm, z[k]);
       } else if (n) {
         zm = fmaxf(zm, z[0]);
-        if (filtered) atomicAdd(&s.n[R.linear_bin(z[0])], 1u);
       }
     });
     packed = (u64)key_of(zm) << 32;
@@ -495,112 +489,127 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   for (int o = 16; o > 0; o >>= 1) packed = max(packed, __shfl_xor_sync(0xffffffffu, packed, o));
   if (lane == 0) s.scan[wid] = packed;
   __syncthreads();
+  // a block's shared memory may be written once it runs
   if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
   if (wid == 0) {
     packed = s.scan[lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) packed = max(packed, __shfl_xor_sync(0xffffffffu, packed, o));
-    if (lane == 0) first.best[rank] = packed;
+    if (lane < blocks) cluster.map_shared_rank(&s, lane)->best[rank] = packed;  // to every block
   }
-  if (rank > 0 && filtered && s.n[tid]) atomicAdd(&first.n[tid], s.n[tid]);
   R.cluster_sync(blocks);
-  // the first block decides which keys may still be kept: [lo, top_key]; of them [lo, hi] hold the border
-  uint32_t lo = kLowest, hi = 0u, threshold = kLowest, ties_n = 0;
-  u64 ahead = 0ull, want = 0ull;
-  bool open = false;  // the k-th largest lies strictly inside [lo, hi]
-  if (rank == 0) {
-    u64 best = s.best[0];
-    for (int r = 1; r < blocks; ++r) best = max(best, s.best[r]);
-    R.set_top((uint32_t)(best >> 32));
-    hi = R.top_key;
-    const bool done = greedy || R.top_key <= kLowest;
-    bool fits = false;
-    if (done) {
-      if (tid == 0) {
-        a.token[row] = greedy ? (int64_t)(0xffffffffu - (uint32_t)best) : 0;
-        a.logprob[row] = greedy ? 0.f : __int_as_float(0x7fffffff);
+  packed = s.best[0];
+  for (int r = 1; r < blocks; ++r) packed = max(packed, s.best[r]);
+  R.set_top((uint32_t)(packed >> 32));
+  if (greedy || R.top_key <= kLowest) {  // alike in every block
+    if (rank == 0 && tid == 0) {
+      a.token[row] = greedy ? (int64_t)(0xffffffffu - (uint32_t)packed) : 0;
+      a.logprob[row] = greedy ? 0.f : __int_as_float(0x7fffffff);
+    }
+    return;
+  }
+  const bool by_count = want_k > 0 && want_k < a.V;
+  bool by_mass = p < 1.0;
+  // below this key exp(z - zmax) < min_p for certain, with room for the logarithm's rounding and that of the sum
+  uint32_t min_cut = kLowest;
+  if (min_p > 0.f)
+    min_cut = max(min(key_of(R.zmax_f + (logf(min_p) - 1e-3f) - fabsf(R.zmax_f) * 1e-6f), R.top_key), kLowest);
+  const int ish = a.index_shift;
+  const double least = (double)min_p * s.table[0];
+  uint32_t lo = kLowest, hi = R.top_key, threshold = kLowest, ties_n = 0;
+  u64 ahead = 0ull, want = 0ull, total = 0ull;
+  u64 ties_in = ~0ull;  // how many keys equal to the threshold are in
+  int tie_last = a.V, route = DRAW;
+  if (by_count || by_mass) {
+    // 2. counts; the sum of all weights where top-p alone decides
+    const bool sum_now = by_mass && !by_count && !(min_p > 0.f);
+    u64 sum = 0ull;
+    R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (k < n) {
+          atomicAdd(&s.n[R.linear_bin(z[k])], 1u);
+          if (sum_now) sum += R.fixed(R.weight(R.key_or_low(z[k])));
+        }
+    });
+    if (sum_now) {
+      sum = R.block_sum(sum);
+      if (tid == 0) first.total[rank] = sum;
+    } else {
+      __syncthreads();
+    }
+    if (rank > 0 && s.n[tid]) atomicAdd(&first.n[tid], s.n[tid]);
+    R.cluster_sync(blocks);
+    // where min-p cuts above top-p's border for certain, top-p decides nothing
+    if (by_mass && !by_count && min_p > 0.f) {
+      if (rank == 0) {
+        R.bracket(-1.0, fmax(p, 0.0), R.linear_bin(value_of(min_cut)));
+        if (tid == 0) s.route = s.bin;
       }
-    } else if (filtered) {
+      R.cluster_sync(blocks);
+      by_mass = first.route == 0;
+      if (by_mass) {
+        u64 m = 0ull;
+        R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            if (k < n) m += R.fixed(R.weight(R.key_or_low(z[k])));
+        });
+        m = R.block_sum(m);
+        if (tid == 0) first.total[rank] = m;
+      }
+      R.cluster_sync(blocks);
+    }
+  }
+  if (by_count || by_mass) {
+    bool open = false;  // the k-th largest lies strictly inside [lo, hi]
+    if (rank == 0) {
       if (by_count) {
         want = (u64)want_k;
         R.template find<false>(0ull, want);
         ahead = s.ahead;
         open = !(s.bin_n == 1u || ahead + s.bin_n == want);
         R.edges(s.bin, s.bin, lo, hi);
-      } else if (by_mass) {
-        R.bracket(fmax(p, 0.0));
+      } else {
+        for (int r = 0; r < blocks; ++r) total += s.total[r];
+        want = (u64)floor(fmax(p, 0.0) * (double)total);
+        R.bracket((double)want, 0.0, 0);
         R.edges(s.bin_lo, max(s.bin_lo, s.bin_hi), lo, hi);
       }
-      if (min_p > 0.f && !by_count) {
-        // exp(z - zmax) >= min_p, with room for the logarithm's rounding and that of the sum
-        const float zmax = value_of(R.top_key);
-        const uint32_t least = key_of(zmax + (logf(min_p) - 1e-3f) - fabsf(zmax) * 1e-6f);
-        lo = max(lo, min(least, R.top_key));
-        hi = max(hi, lo);
+      const int last = R.linear_bin(value_of(lo)), past = R.linear_bin(value_of(hi));
+      const u64 all = R.block_sum(tid <= last ? s.n[tid] : 0u);
+      const u64 border = R.block_sum(tid <= last && tid >= past ? s.n[tid] : 0u);
+      // a long list is drawn from by one block, the row by all
+      const u64 most = by_count ? (u64)a.list_cap : min((u64)a.list_cap, (u64)(4 * kThreads));
+      route = all <= most ? LIST_ALL : !by_count && border <= (u64)a.list_cap ? LIST_BORDER : ALONE;
+      if (tid == 0) {
+        s.lo = lo;
+        s.hi = hi;
+        s.route = route;
       }
-      const int last = R.linear_bin(value_of(lo));
-      fits = R.block_sum(tid <= last ? s.n[tid] : 0u) <= (u64)a.list_cap;
     }
-    if (tid == 0) {
-      s.top_key = R.top_key;
-      s.lo = lo;
-      s.done = done;
-      s.listing = fits;
-      s.summing = by_mass && !by_count;
+    R.cluster_sync(blocks);
+    if (rank > 0) {
+      lo = first.lo;
+      hi = first.hi;
+      route = first.route;
     }
-  }
-  R.cluster_sync(blocks);
-  if (first.done) {
-    R.cluster_sync(blocks);  // nobody leaves while `first` is read
-    return;
-  }
-  const bool listing = first.listing, summing = first.summing;
-  if (rank > 0) {
-    R.set_top(first.top_key);
-    lo = first.lo;
-  }
-  const int ish = a.index_shift;
-  const double least = (double)min_p * s.table[0];
-  // second pass: the list of keys >= lo and the sum of all weights; without a filter, the weight of each index bin
-  if (!filtered) {
-    R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
+    // 3. the list, and the weight in front of it
+    if (route != ALONE) {
+      const float lo_z = value_of(lo), hi_z = route == LIST_ALL ? INFINITY : value_of(hi);
+      const float sum_z = by_count ? INFINITY : value_of(hi);
+      const bool all_in = lo <= kLowest;
       u64 m = 0ull;
-      int b = i >> ish;
-#pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        if (k < n) {
-          if ((i + k) >> ish != b) {  // bins shorter than a vector
-            if (m) R.add_mass(b, m);
-            m = 0ull;
-            b = (i + k) >> ish;
-          }
-          m += R.fixed(R.weight(R.key_or_low(z[k])));
-        }
-      if (m) R.add_mass(b, m);
-    });
-    __syncthreads();
-    if (rank > 0) {  // the bins of a block's part are its own
-      const int b = (i0 >> ish) + tid;
-      if (i0 < i1 && b <= (i1 - 1) >> ish) {
-        first.m0[b] = s.m0[b];
-        first.m1[b] = s.m1[b];
-        first.m2[b] = s.m2[b];
-      }
-    }
-  } else if (listing || summing) {
-    const float lo_z = value_of(lo);
-    const bool all_in = lo <= kLowest;
-    u64 sum = 0ull;
-    R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
-      if (summing) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          if (k < n) sum += R.fixed(R.weight(R.key_or_low(z[k])));
-      }
-      if (listing) {
+      R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
         int c = 0;
+        unsigned in = 0u;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) c += k < n && (z[k] >= lo_z || all_in);
+        for (int k = 0; k < VEC; ++k) {
+          const bool on = k < n && ((z[k] >= lo_z && z[k] <= hi_z) || (all_in && !(z[k] > hi_z)));
+          c += on;
+          in |= (unsigned)on << k;
+          if (k < n && z[k] > sum_z) m += R.fixed(R.weight(key_of(z[k])));
+        }
         if (__any_sync(0xffffffffu, c > 0)) {
           const int incl = warp_scan(c);
           int at = 0;
@@ -608,52 +617,43 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
           at = __shfl_sync(0xffffffffu, at, 31) + incl - c;
 #pragma unroll
           for (int k = 0; k < VEC; ++k)
-            if (k < n && (z[k] >= lo_z || all_in)) first_list[at++] = make_uint2(R.key_or_low(z[k]), (uint32_t)(i + k));
+            if (in >> k & 1u) first_list[at++] = make_uint2(R.key_or_low(z[k]), (uint32_t)(i + k));
+        }
+      });
+      m = R.block_sum(m);
+      if (tid == 0) first.total[rank] = m;
+    }
+    R.cluster_sync(blocks);
+    if (rank > 0 && route == LIST_ALL) return;  // the rest is the first block's alone
+    if (rank == 0) {
+      R.listed = route != ALONE;
+      if (by_count) {
+        threshold = open ? R.template narrow<false>(lo, hi, want, ahead, ties_n, false) : lo;
+        if (by_mass) {
+          lo = threshold;
+          hi = R.top_key;
+          u64 m = 0ull;
+          R.each([&](uint32_t key, int) {
+            if (key >= lo) m += R.fixed(R.weight(key));
+          });
+          total = R.block_sum(m);
+          want = (u64)floor(fmax(p, 0.0) * (double)total);
         }
       }
-    });
-    if (summing) {
-      sum = R.block_sum(sum);
-      if (tid == 0) first.total[rank] = sum;
-    }
-  }
-  R.cluster_sync(blocks);
-  if (rank > 0) return;  // the rest is the first block's alone
-  u64 total = 0ull;
-  if (by_mass && !by_count)
-    for (int r = 0; r < blocks; ++r) total += s.total[r];
-  R.listed = listing;
-  if (by_count) threshold = open ? R.template narrow<false>(lo, hi, want, ahead, ties_n, false) : lo;
-  u64 ties_in = ~0ull;  // how many keys equal to the threshold are in
-  if (by_mass) {
-    const bool whole = hi == R.top_key;  // nothing lies in front of [lo, hi]
-    if (by_count) {
-      lo = threshold;
-      hi = R.top_key;
-    }
-    u64 inside = 0ull;
-    if (by_count || min_p > 0.f) {
-      R.each([&](uint32_t key, int) {
-        if (key >= lo) inside += R.fixed(R.weight(key));
-      });
-      inside = R.block_sum(inside);
-    }
-    if (by_count) total = inside;
-    want = (u64)floor(fmax(p, 0.0) * (double)total);
-    ahead = 0ull;
-    if (!by_count && min_p > 0.f && inside <= want) {
-      threshold = lo;  // min-p cuts in front of the nucleus' border
-    } else {
-      threshold = R.template narrow<true>(lo, hi, want, ahead, ties_n, !by_count && !whole);
-      if (ties_n > 1) {
-        ties_in = (want - ahead) / R.fixed(R.weight(threshold)) + 1ull;  // weight > 0: the sum crosses within these ties
-        if (ties_in >= ties_n) ties_in = ~0ull;
+      if (by_mass) {
+        ahead = 0ull;
+        if (!by_count && R.listed)
+          for (int r = 0; r < blocks; ++r) ahead += s.total[r];
+        threshold = R.template narrow<true>(lo, hi, want, ahead, ties_n, !by_count && !R.listed);
+        if (ties_n > 1) {
+          ties_in = (want - ahead) / R.fixed(R.weight(threshold)) + 1ull;  // weight > 0: the sum crosses within these ties
+          if (ties_in >= ties_n) ties_in = ~0ull;
+        }
       }
     }
   }
   // of the threshold's ties those up to this index
-  int tie_last = a.V;
-  if (ties_in != ~0ull) {
+  if (ties_in != ~0ull) {  // (the first block alone comes here)
     __syncthreads();
     R.template clear<false>();
     R.each([&](uint32_t key, int i) {
@@ -670,12 +670,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     tie_last = s.at;
   }
   auto kept = [&](uint32_t key, int i) -> u64 {
-    if (key < threshold || key == 0u || (key == threshold && i > tie_last)) return 0ull;
+    if (key < threshold || key < min_cut || (key == threshold && i > tie_last)) return 0ull;
     const double w = R.weight(key);
     return w >= least ? R.fixed(w) : 0ull;
   };
-  // the draw: kept weight by index
-  if (filtered) {
+  // 4. the draw: kept weight by index
+  if (route == LIST_ALL) {
     __syncthreads();
     R.template clear<true>();
     R.each([&](uint32_t key, int i) {
@@ -683,6 +683,50 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       if (m) R.add_mass(i >> ish, m);
     });
     __syncthreads();
+  } else {
+    if (by_count || by_mass) {
+      if (rank == 0) {
+        __syncthreads();
+        R.template clear<true>();
+        if (tid == 0) {
+          s.threshold = threshold;
+          s.tie_last = tie_last;
+        }
+      }
+      R.cluster_sync(blocks);
+      if (rank > 0) {
+        threshold = first.threshold;
+        tie_last = first.tie_last;
+      }
+    }
+    const uint32_t from = max(threshold, min_cut);
+    const float cut = value_of(from);
+    R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
+      u64 m = 0ull;
+      int b = i >> ish;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (k < n && (z[k] >= cut || from <= kLowest)) {
+          if ((i + k) >> ish != b) {  // bins shorter than a vector
+            if (m) R.add_mass(b, m);
+            m = 0ull;
+            b = (i + k) >> ish;
+          }
+          m += kept(R.key_or_low(z[k]), i + k);
+        }
+      if (m) R.add_mass(b, m);
+    });
+    __syncthreads();
+    if (rank > 0) {  // the bins of a block's part are its own
+      const int b = (i0 >> ish) + tid;
+      if (i0 < i1 && b <= (i1 - 1) >> ish) {
+        first.m0[b] = s.m0[b];
+        first.m1[b] = s.m1[b];
+        first.m2[b] = s.m2[b];
+      }
+    }
+    R.cluster_sync(blocks);
+    if (rank > 0) return;
   }
   u64 sum = R.bin_mass(tid), all;
   const u64 run = R.block_before(sum, all);
