@@ -128,14 +128,16 @@ struct Row {
   float div, pen;
   bool vec;           // 8-byte loads
   bool plain;         // z is the logit
+  bool penalised;
   bool listed = false;
-  float zmax_f = 0.f;
+  float zmax_f = 0.f, bin_top = 0.f;
   uint32_t top_key = 0u;
   double zmax = 0.0;
 
   __device__ __forceinline__ void set_top(uint32_t key) {
     top_key = key;
     zmax_f = value_of(key);
+    bin_top = fminf(zmax_f, 3.4028234e38f);  // an infinite maximum is in bin 0 too
     zmax = (double)zmax_f;
   }
   static __device__ __forceinline__ void cluster_sync(int blocks) {
@@ -147,11 +149,8 @@ struct Row {
 
   // z of an element: -0 becomes 0; NaN stays NaN (its key is that of -inf)
   __device__ __forceinline__ float scaled(float logit, int i) const {
-    float z = logit;
-    if (!plain) {
-      z = __fdiv_rn(z, div);
-      if (a.seen && (seen_bits[i >> 5] >> (i & 31) & 1u)) z = __fdiv_rn(z, pen);
-    }
+    float z = div == 1.f ? logit : __fdiv_rn(logit, div);
+    if (penalised && (seen_bits[i >> 5] >> (i & 31) & 1u)) z = __fdiv_rn(z, pen);
     return z + 0.f;
   }
   static __device__ __forceinline__ uint32_t key_or_low(float z) { return isnan(z) ? kLowest : key_of(z); }
@@ -160,43 +159,51 @@ struct Row {
   // f(z[VEC], index of the first, how many) for groups of elements of [i0, i1);
   // the lanes of a warp call it together (none behind the end).
   template <typename F> __device__ __forceinline__ void groups(int i0, int i1, F f) const {
-    // Short loop bodies: a pass runs over them a few times only.  Four vectors are in flight a thread.
+    if (plain)
+      groups_of<false>(i0, i1, f);
+    else
+      groups_of<true>(i0, i1, f);
+  }
+  template <bool SCALE, typename F> __device__ __forceinline__ void groups_of(int i0, int i1, F f) const {
+    // Four vectors in flight a thread, each register reloaded as soon as it is
+    // used (moving them along would wait for the loads).  Whole blocks of
+    // vectors first, so that the loop over them checks nothing.
     constexpr int AHEAD = 4;
     int rest = i0;
     if (vec) {
-      const int v0 = i0 / VEC, v1 = i1 / VEC;  // i0 is a multiple of VEC
-      const uint2* src = reinterpret_cast<const uint2*>(lr);
+      const int v0 = i0 / VEC + threadIdx.x;  // i0 is a multiple of VEC
+      const int full = (i1 / VEC - i0 / VEC) / kThreads;
+      const uint2* src = reinterpret_cast<const uint2*>(lr) + v0;
       uint2 x[AHEAD];
 #pragma unroll
-      for (int q = 0; q < AHEAD; ++q) {
-        const int v = v0 + q * kThreads + threadIdx.x;
-        x[q] = v < v1 ? src[v] : make_uint2(0u, 0u);
-      }
+      for (int q = 0; q < AHEAD; ++q)
+        if (q < full) x[q] = src[q * kThreads];
 #pragma unroll 1
-      for (int b = v0; b < v1; b += kThreads) {
-        const int v = b + threadIdx.x;
-        union { uint2 raw; T e[VEC]; } cur;
-        cur.raw = x[0];
+      for (int b = 0; b < full; b += AHEAD) {
 #pragma unroll
-        for (int q = 0; q + 1 < AHEAD; ++q) x[q] = x[q + 1];
-        const int next = v + AHEAD * kThreads;
-        if (next < v1) x[AHEAD - 1] = src[next];
-        float z[VEC];
+        for (int q = 0; q < AHEAD; ++q) {
+          if (b + q >= full) break;
+          union { uint2 raw; T e[VEC]; } cur;
+          cur.raw = x[q];
+          if (b + q + AHEAD < full) x[q] = src[(b + q + AHEAD) * kThreads];
+          const int i = (v0 + (b + q) * kThreads) * VEC;
+          float z[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) z[k] = v < v1 ? scaled(to_f<T>(cur.e[k]), v * VEC + k) : 0.f;
-        f(z, v * VEC, v < v1 ? VEC : 0);
+          for (int k = 0; k < VEC; ++k) z[k] = SCALE ? scaled(to_f<T>(cur.e[k]), i + k) : to_f<T>(cur.e[k]) + 0.f;
+          f(z, i, VEC);
+        }
       }
-      rest = v1 * VEC;
+      rest = i0 + full * kThreads * VEC;
     }
-    // the tail, and rows that are not aligned
+    // the rest, and rows that are not aligned
 #pragma unroll 1
-    for (int b = rest; b < i1; b += kThreads) {
-      const int i = b + threadIdx.x;
+    for (int b = rest; b < i1; b += kThreads * VEC) {
       float z[VEC];
+      const int i = b + threadIdx.x * VEC;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) z[k] = 0.f;
-      if (i < i1) z[0] = scaled(to_f<T>(lr[i]), i);
-      f(z, i, i < i1 ? 1 : 0);
+      for (int k = 0; k < VEC; ++k)
+        z[k] = i + k < i1 ? (SCALE ? scaled(to_f<T>(lr[i + k]), i + k) : to_f<T>(lr[i + k]) + 0.f) : 0.f;
+      f(z, i, max(0, min(VEC, i1 - i)));
     }
   }
   // f(key, index) for every element of the list, or of the row; the lanes of a warp call it together (key 0: none).
@@ -222,12 +229,17 @@ struct Row {
   // series to r^6 (|r| <= 0.022: 5e-16 beyond it).  Sixteen doubles fill the
   // shared-memory banks once, so lanes never wait for one another (a table of
   // 256 with a shorter series did: 20 against 9 us for a row of 32000).
+  // Without branches, so that the chains of a vector's elements overlap.
   __device__ __forceinline__ double weight(uint32_t key) const {
-    if (key == top_key) return s.table[0];
-    return weight_at((double)value_of(key) - zmax);
+    // the fp32 value as a double by its bits (a conversion takes eight times an
+    // fp64 operation): zero and denormals come out below 2^-126, infinity as
+    // 2^128, which is all the same to the difference
+    const uint32_t b = __float_as_uint(value_of(key));
+    const double v = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+    return weight_at(key == top_key ? 0.0 : v - zmax);
   }
   __device__ __forceinline__ double weight_at(double x) const {
-    if (!(x > -50.0)) return 0.0;  // below 2^-72
+    x = x > -60.0 ? x : -60.0;  // 2^-86: 0 once rounded
     const double t = fma(x, 23.083120654223414, 6755399441055744.0);  // 16 / ln 2; 1.5 * 2^52 rounds to an integer
     const int k = __double2loint(t);
     const double r = fma(t - 6755399441055744.0, -0.04332169878499658, x);  // ln 2 / 16
@@ -247,8 +259,7 @@ struct Row {
 
   // bins of the counts: bin b is within 1/64 of zmax - b / 32; the last (with NaN) is open
   __device__ __forceinline__ int linear_bin(float z) const {
-    const float d = z == zmax_f ? 0.f : zmax_f - z;  // (both may be infinite)
-    const float b = fminf(d * 32.f, (float)(kBins - 1));
+    const float b = fmaxf(fminf((bin_top - z) * 32.f, (float)(kBins - 1)), 0.f);
     return __float_as_int(b + 8388608.f) & (kBins - 1);  // 2^23 rounds to an integer
   }
 
@@ -265,6 +276,17 @@ struct Row {
   }
   __device__ __forceinline__ u64 bin_mass(int b) const {
     return (u64)s.m0[b] + ((u64)s.m1[b] << a.limb) + ((u64)s.m2[b] << 2 * a.limb);
+  }
+  // Adds each lane's weight of its elements, whose indices follow the lane's, to
+  // their index bin; the lanes of a bin (a power of two) add up first.
+  __device__ __forceinline__ void add_by_index(int i, u64 m) {
+    const int lanes = min((1 << a.index_shift) / VEC, 32);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      if (o >= lanes) break;
+      m += __shfl_xor_sync(0xffffffffu, m, o);
+    }
+    if (m && (threadIdx.x & (lanes - 1)) == 0) add_mass(i >> a.index_shift, m);
   }
   // Adds the elements `in` to bins b; a warp whose elements share a bin (equal logits) adds once.
   __device__ __forceinline__ void add(bool in, int b, u64 m) {
@@ -450,12 +472,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   const bool greedy = !(temp > 0.f);
   const T* lr = (const T*)a.logits + row * a.ls;
   Row<T> R{a, s, seen_bits, list, lr, greedy ? 1.f : temp, pen, ((uintptr_t)lr & 7) == 0,
-           (greedy || temp == 1.f) && (a.seen == nullptr || pen == 1.f)};
+           (greedy || temp == 1.f) && (a.seen == nullptr || pen == 1.f), a.seen != nullptr && pen != 1.f};
   if (blocks > 1) asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
   if (tid < kTable) s.table[tid] = ldexp(exp2((double)tid / kTable), a.fbits);
   s.n[tid] = s.m0[tid] = s.m1[tid] = s.m2[tid] = 0u;
   if (tid == 0) s.list_n = s.bin = 0;
-  if (a.seen && !R.plain) {
+  if (R.penalised) {
     for (int i = tid; i < seen_words; i += kThreads) seen_bits[i] = 0u;
     __syncthreads();
     for (int i = tid; i < a.L; i += kThreads) {
@@ -476,12 +498,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   } else {
     float zm = -INFINITY;
     R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
-      if (n == VEC) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) zm = fmaxf(zm, z[k]);
-      } else if (n) {
-        zm = fmaxf(zm, z[0]);
-      }
+      for (int k = 0; k < VEC; ++k)
+        if (k < n) zm = fmaxf(zm, z[k]);
     });
     packed = (u64)key_of(zm) << 32;
   }
@@ -520,16 +539,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   u64 ahead = 0ull, want = 0ull, total = 0ull;
   u64 ties_in = ~0ull;  // how many keys equal to the threshold are in
   int tie_last = a.V, route = DRAW;
-  if (by_count || by_mass) {
+  const bool filtered = by_count || by_mass || min_p > 0.f;
+  if (filtered) {
     // 2. counts; the sum of all weights where top-p alone decides
     const bool sum_now = by_mass && !by_count && !(min_p > 0.f);
     u64 sum = 0ull;
     R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (k < n) {
-          atomicAdd(&s.n[R.linear_bin(z[k])], 1u);
-          if (sum_now) sum += R.fixed(R.weight(R.key_or_low(z[k])));
+        if (k < n) atomicAdd(&s.n[R.linear_bin(z[k])], 1u);
+      if (sum_now)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const u64 w = R.fixed(R.weight(R.key_or_low(z[k])));
+          sum += k < n ? w : 0ull;
         }
     });
     if (sum_now) {
@@ -552,8 +575,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         u64 m = 0ull;
         R.groups(i0, i1, [&](const float (&z)[VEC], int, int n) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k)
-            if (k < n) m += R.fixed(R.weight(R.key_or_low(z[k])));
+          for (int k = 0; k < VEC; ++k) {
+            const u64 w = R.fixed(R.weight(R.key_or_low(z[k])));
+            m += k < n ? w : 0ull;
+          }
         });
         m = R.block_sum(m);
         if (tid == 0) first.total[rank] = m;
@@ -561,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       R.cluster_sync(blocks);
     }
   }
-  if (by_count || by_mass) {
+  if (filtered) {
     bool open = false;  // the k-th largest lies strictly inside [lo, hi]
     if (rank == 0) {
       if (by_count) {
@@ -570,6 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         ahead = s.ahead;
         open = !(s.bin_n == 1u || ahead + s.bin_n == want);
         R.edges(s.bin, s.bin, lo, hi);
+      } else if (!by_mass) {  // min-p alone
+        lo = min_cut;
       } else {
         for (int r = 0; r < blocks; ++r) total += s.total[r];
         want = (u64)floor(fmax(p, 0.0) * (double)total);
@@ -581,7 +608,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       const u64 border = R.block_sum(tid <= last && tid >= past ? s.n[tid] : 0u);
       // a long list is drawn from by one block, the row by all
       const u64 most = by_count ? (u64)a.list_cap : min((u64)a.list_cap, (u64)(4 * kThreads));
-      route = all <= most ? LIST_ALL : !by_count && border <= (u64)a.list_cap ? LIST_BORDER : ALONE;
+      route = all <= most                                            ? LIST_ALL
+              : !by_count && !by_mass                                ? DRAW
+              : !by_count && border <= (u64)a.list_cap ? LIST_BORDER : ALONE;
       if (tid == 0) {
         s.lo = lo;
         s.hi = hi;
@@ -595,30 +624,25 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       route = first.route;
     }
     // 3. the list, and the weight in front of it
-    if (route != ALONE) {
+    if (route == LIST_ALL || route == LIST_BORDER) {
       const float lo_z = value_of(lo), hi_z = route == LIST_ALL ? INFINITY : value_of(hi);
-      const float sum_z = by_count ? INFINITY : value_of(hi);
+      const float sum_z = by_mass && !by_count ? value_of(hi) : INFINITY;
       const bool all_in = lo <= kLowest;
       u64 m = 0ull;
       R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
-        int c = 0;
-        unsigned in = 0u;
+        bool over = false;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const bool on = k < n && ((z[k] >= lo_z && z[k] <= hi_z) || (all_in && !(z[k] > hi_z)));
-          c += on;
-          in |= (unsigned)on << k;
-          if (k < n && z[k] > sum_z) m += R.fixed(R.weight(key_of(z[k])));
+          if (k < n && ((z[k] >= lo_z && z[k] <= hi_z) || (all_in && !(z[k] > hi_z))))  // few elements are
+            first_list[atomicAdd(&first.list_n, 1)] = make_uint2(R.key_or_low(z[k]), (uint32_t)(i + k));
+          over |= k < n && z[k] > sum_z;
         }
-        if (__any_sync(0xffffffffu, c > 0)) {
-          const int incl = warp_scan(c);
-          int at = 0;
-          if (lane == 31) at = atomicAdd(&first.list_n, incl);
-          at = __shfl_sync(0xffffffffu, at, 31) + incl - c;
+        if (__any_sync(0xffffffffu, over))
 #pragma unroll
-          for (int k = 0; k < VEC; ++k)
-            if (in >> k & 1u) first_list[at++] = make_uint2(R.key_or_low(z[k]), (uint32_t)(i + k));
-        }
+          for (int k = 0; k < VEC; ++k) {
+            const u64 w = R.fixed(R.weight(key_of(z[k])));
+            m += k < n && z[k] > sum_z ? w : 0ull;
+          }
       });
       m = R.block_sum(m);
       if (tid == 0) first.total[rank] = m;
@@ -626,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     R.cluster_sync(blocks);
     if (rank > 0 && route == LIST_ALL) return;  // the rest is the first block's alone
     if (rank == 0) {
-      R.listed = route != ALONE;
+      R.listed = route == LIST_ALL || route == LIST_BORDER;
       if (by_count) {
         threshold = open ? R.template narrow<false>(lo, hi, want, ahead, ties_n, false) : lo;
         if (by_mass) {
@@ -670,9 +694,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     tie_last = s.at;
   }
   auto kept = [&](uint32_t key, int i) -> u64 {
-    if (key < threshold || key < min_cut || (key == threshold && i > tie_last)) return 0ull;
     const double w = R.weight(key);
-    return w >= least ? R.fixed(w) : 0ull;
+    const bool in = key >= threshold && key >= min_cut && !(key == threshold && i > tie_last) && w >= least;
+    return in ? R.fixed(w) : 0ull;
   };
   // 4. the draw: kept weight by index
   if (route == LIST_ALL) {
@@ -684,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     });
     __syncthreads();
   } else {
-    if (by_count || by_mass) {
+    if (filtered) {
       if (rank == 0) {
         __syncthreads();
         R.template clear<true>();
@@ -701,20 +725,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     }
     const uint32_t from = max(threshold, min_cut);
     const float cut = value_of(from);
+    // a vector lies in one index bin, and a warp's vectors follow one another
+    const bool aligned = ish >= 2 && (i0 & (VEC - 1)) == 0;
+    const bool everything = from <= kLowest;
     R.groups(i0, i1, [&](const float (&z)[VEC], int i, int n) {
+      bool hit = everything;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) hit |= k < n && z[k] >= cut;
+      if (!__any_sync(0xffffffffu, hit)) return;
       u64 m = 0ull;
-      int b = i >> ish;
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (k < n && (z[k] >= cut || from <= kLowest)) {
-          if ((i + k) >> ish != b) {  // bins shorter than a vector
-            if (m) R.add_mass(b, m);
-            m = 0ull;
-            b = (i + k) >> ish;
-          }
-          m += kept(R.key_or_low(z[k]), i + k);
-        }
-      if (m) R.add_mass(b, m);
+      {
+        u64 w = kept(R.key_or_low(z[k]), i + k);
+        w = k < n ? w : 0ull;
+        if (!aligned && w) R.add_mass((i + k) >> ish, w);
+        m += w;
+      }
+      if (aligned) R.add_by_index(i, m);  // by every lane
     });
     __syncthreads();
     if (rank > 0) {  // the bins of a block's part are its own
