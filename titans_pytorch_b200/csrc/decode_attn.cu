@@ -252,6 +252,481 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const float* __re
   if (lse && lane == 0) lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
+// ------------------------------------------------------------- tensor cores
+// Queries in bf16 or fp16 over keys of the same type or of 8 bits.
+//
+// A warp takes 16 keys at a time against 8 * NQ query rows, as S^T = K Q^T and
+// O^T += V^T P^T on mma.m16n8k16: keys (then head dimensions) are the 16 rows,
+// queries the 8 columns, so a single query wastes little.  The order of the
+// contracted index is free, so each lane loads whole 16-byte pieces of its key
+// rows straight from memory into operand registers (no shared memory): lane
+// (r, c) = (lane / 4, lane % 4) holds keys r and r + 8, pieces c of 8 (16 at 8
+// bits) dimensions.  For V the lane holds the four keys 2c, 2c+1, 2c+8, 2c+9 and
+// piece r; byte permutes pair up neighbouring keys.  P passes from the score
+// layout to the operand layout by an 8x8 transpose in registers.
+//
+// Bound by memory: decoding reads every key once for a handful of queries, far
+// below the tensor cores' rate even at mma.sync's, so tcgen05 with its 128-row
+// tiles would gain nothing.  K registers are reloaded as soon as the scores have
+// read them, V registers after the product, so each warp keeps 4 to 8 KB in
+// flight.
+//
+// The running maximum moves only when a score exceeds it by more than 8 (in
+// log2): weights stay below 2^8, and most steps need no exchange between lanes.
+// 8-bit values are exact in bf16; their scale is multiplied into the weight, in
+// bf16 for its range.  Weights are rounded to 16 bits for the product (half a
+// step each); sums of them are taken before that, in fp32.
+
+template <typename T> struct Pair;  // two packed 16-bit floats
+template <> struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Pair<__half> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Bytes 0 and 2 of p as two numbers of the cache's type, in T, exactly.
+template <typename C, typename T> __device__ __forceinline__ uint32_t widen(uint32_t p);
+// int8 in bf16: 128 + (b & 127) less 128 + (b & 128)
+template <> __device__ __forceinline__ uint32_t widen<int8_t, __nv_bfloat16>(uint32_t p) {
+  const uint32_t x = (p & 0x007f007fu) | 0x43004300u, y = (p & 0x00800080u) | 0x43004300u;
+  __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// int8 in fp16: 1024 + (b + 128) less 1152
+template <> __device__ __forceinline__ uint32_t widen<int8_t, __half>(uint32_t p) {
+  const uint32_t x = ((p & 0x00ff00ffu) ^ 0x00800080u) | 0x64006400u, y = 0x64806480u;
+  __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// e4m3 in bf16: the same bits four places down are the number times 2^-120
+template <> __device__ __forceinline__ uint32_t widen<e4m3, __nv_bfloat16>(uint32_t p) {
+  const uint32_t x = ((p & 0x00800080u) << 8) | ((p & 0x007f007fu) << 4), y = 0x7b807b80u;
+  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// e4m3 in fp16: one place down from the high byte, times 2^8
+template <> __device__ __forceinline__ uint32_t widen<e4m3, __half>(uint32_t p) {
+  const uint32_t x = ((p & 0x00800080u) << 8) | ((p & 0x007f007fu) << 7), y = 0x5c005c00u;
+  __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+template <typename C, int D> struct Layout {
+  static constexpr bool k16 = sizeof(C) == 2;
+  static constexpr int CK = k16 ? 8 : D % 64 == 0 ? 16 : 8;             // dimensions in a lane's piece of a key
+  static constexpr int CV = k16 ? (D % 64 == 0 ? 8 : 4) : D == 128 ? 16 : D == 64 ? 8 : 4;  // of a value
+  static constexpr int KW = D / 4 * sizeof(C) / 4;                     // words of a key a lane holds
+  static constexpr int VW = D / 8 * sizeof(C) / 4;                     // words of a value (may end mid-word at D = 96)
+  static constexpr int U = D == 64 ? (k16 ? 2 : 4) : k16 ? 1 : 2;       // groups of 16 keys a step
+};
+
+template <int BYTES> __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
+  if constexpr (BYTES == 16) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    w[0] = a.x; w[1] = a.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+struct MmaArgs {
+  KeySource cache;
+  const void* q;
+  int64_t sqb, sqh;
+  float* part;
+  void* out;       // written directly when a row has one piece in all
+  float* lse;
+  int splits, split0, nsplit;
+  int Hq, group, rows, tiles;  // query rows of a key head in this launch; tiles of them
+  int warps_row;               // warps side by side over rows; the others split the keys
+  bool shared;                 // rows run over the whole batch (prefix alone)
+  float scale_log2;
+};
+
+template <typename T, int D, int NQ>
+struct Warp {
+  static constexpr int STEPS = D / 16, R = 8 * NQ;
+  uint32_t q[NQ][STEPS][2];
+  float o[NQ][STEPS][4];  // [dimension tile][d r / r + 8, query 2c / 2c + 1]
+  float m[NQ][2], l[NQ][2];
+  int r, c;
+
+  // One kind of keys [lo, hi), every stride-th block of 16 U starting at `block`.
+  template <typename C>
+  __device__ __forceinline__ void run(const KeySource& s, int b, int hk, int first, int lo, int hi, int block, int stride,
+                                      float scale) {
+    using L = Layout<C, D>;
+    using TV = typename std::conditional<L::k16, T, __nv_bfloat16>::type;
+    constexpr int U = NQ == 1 ? L::U : 1, KEYS = 16 * U;
+    constexpr int NK = L::KW * 4 / (L::CK * (int)sizeof(C)), NV = D / (8 * L::CV);  // pieces
+    constexpr int KB = L::CK * sizeof(C), VB = L::CV * sizeof(C), VWP = VB / 4;
+    const C* kb = (const C*)s.k.data + b * s.k.sb + hk * s.k.sh + c * L::CK;
+    const C* vb = (const C*)s.v.data + b * s.v.sb + hk * s.v.sh + r * L::CV;
+    uint32_t kw[U][2][L::KW], vw[U][4][NV * VWP];
+    float ks[U][2], vs[U][2];
+    auto slot_of = [&](int i) {
+      int x = first + i;
+      return x >= s.S ? x - s.S : x;
+    };
+    auto load_k = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = base + 16 * u + 8 * h + r;
+          if (i < hi) {
+            const int64_t slot = slot_of(i);
+            const C* p = kb + slot * s.k.ss;
+#pragma unroll
+            for (int j = 0; j < NK; ++j) load_words<KB>(p + j * 4 * L::CK, &kw[u][h][j * (KB / 4)]);
+            if constexpr (CacheTraits<C>::scaled) {
+              ks[u][h] = s.k.scale[b * s.k.qb + hk * s.k.qh + slot * s.k.qs];
+              vs[u][h] = s.v.scale[b * s.v.qb + hk * s.v.qh + slot * s.v.qs];
+            }
+          }
+        }
+    };
+    auto load_v = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = base + 16 * u + 2 * c + (x & 1) + 8 * (x >> 1);
+          if (i < hi) {
+            const C* p = vb + (int64_t)slot_of(i) * s.v.ss;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) load_words<VB>(p + j * 8 * L::CV, &vw[u][x][j * VWP]);
+          } else {  // a weight of zero times whatever the slot holds has to be zero
+#pragma unroll
+            for (int j = 0; j < NV * VWP; ++j) vw[u][x][j] = 0u;
+          }
+        }
+    };
+    int base = lo + block * KEYS;
+    if (base >= hi) return;
+    load_k(base);
+    load_v(base);
+    while (true) {
+      float sc[U][NQ][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[u][n][e] = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+          uint32_t f[2][2];  // [key half][pair]
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (L::k16) {
+              f[h][0] = kw[u][h][2 * t];
+              f[h][1] = kw[u][h][2 * t + 1];
+            } else {
+              const uint32_t w = kw[u][h][t];
+              f[h][0] = widen<C, T>(__byte_perm(w, 0u, 0x4140));
+              f[h][1] = widen<C, T>(__byte_perm(w, 0u, 0x4342));
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) Pair<T>::mma(sc[u][n], f[0][0], f[1][0], f[0][1], f[1][1], q[n][t][0], q[n][t][1]);
+        }
+      float vscale[U][2];
+      float grow = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool in = base + 16 * u + 8 * h + r < hi;
+          float f = scale;
+          if constexpr (CacheTraits<C>::scaled) {
+            f *= ks[u][h];
+            vscale[u][h] = in ? vs[u][h] : 0.f;
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = sc[u][n][2 * h + e];
+              x = in ? x * f : -INFINITY;
+              grow = fmaxf(grow, x - m[n][e]);
+            }
+        }
+      const int next = base + stride * KEYS;
+      const bool more = next < hi;
+      if (more) load_k(next);
+      // m = -inf at first: -inf - -inf is NaN and does not count, a finite score does
+      if (__any_sync(0xffffffffu, grow > 8.f)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = m[n][e];
+#pragma unroll
+            for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(sc[u][n][e], sc[u][n][2 + e]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float corr = mx == m[n][e] ? 1.f : ex2(m[n][e] - mx);
+            m[n][e] = mx;
+            l[n][e] *= corr;
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) {
+              o[n][t][e] *= corr;
+              o[n][t][2 + e] *= corr;
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint32_t p[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              w[e] = ex2(sc[u][n][2 * h + e] - (m[n][e] == -INFINITY ? 0.f : m[n][e]));
+              l[n][e] += w[e];
+              if constexpr (CacheTraits<C>::scaled) w[e] *= vscale[u][h];
+            }
+            p[n][h] = transpose8x8(Pair<TV>::pack(w[0], w[1]));
+          }
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+          uint32_t f[2][2];  // [tile half][key pair]
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int nt = 2 * t + h, e = nt % L::CV, j = nt / L::CV;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              if constexpr (L::k16) {
+                const int w = j * VWP + e / 2;
+                f[h][y] = __byte_perm(vw[u][2 * y][w], vw[u][2 * y + 1][w], e & 1 ? 0x7632 : 0x5410);
+              } else {
+                const int w = j * VWP + e / 4;
+                // byte e of the two keys to bytes 0 and 2
+                f[h][y] = widen<C, TV>(
+                    __byte_perm(vw[u][2 * y][w], vw[u][2 * y + 1][w], 0x0000 | (e & 3) | ((4 + (e & 3)) << 8)));
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) Pair<TV>::mma(o[n][t], f[0][0], f[1][0], f[0][1], f[1][1], p[n][0], p[n][1]);
+        }
+      }
+      if (!more) break;
+      load_v(next);
+      base = next;
+    }
+  }
+};
+
+template <typename T, typename C, int D, int NQ>
+__global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(MmaArgs a) {
+  using W = Warp<T, D, NQ>;
+  constexpr int R = W::R, STEPS = W::STEPS;
+  extern __shared__ float sm[];  // [warp][R][D + 2]: O, m, l (row stride odd against bank conflicts of the transposed store)
+  constexpr int RS = D + 3;
+  const int split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wr = warp % a.warps_row, wk = warp / a.warps_row, nk = kWarps / a.warps_row;
+  const int row0 = (tile * a.warps_row + wr) * R;
+  W w;
+  w.r = lane >> 2;
+  w.c = lane & 3;
+  // row -> (sequence, query head)
+  auto place = [&](int row, int& bb, int& h) {
+    bb = a.shared ? row / a.group : b;
+    h = hk * a.group + (a.shared ? row - bb * a.group : row);
+  };
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = row0 + 8 * n + w.r;
+    int bb = 0, h = 0;
+    if (row < a.rows) place(row, bb, h);
+    const T* qp = (const T*)a.q + bb * a.sqb + h * a.sqh;
+    // in the order of the dimensions that the keys' pieces have
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        constexpr int CK = Layout<C, D>::CK;
+        const int d = (t / (CK / 4)) * 4 * CK + w.c * CK + (t % (CK / 4)) * 4 + 2 * y;
+        float e0 = 0.f, e1 = 0.f;
+        if (row < a.rows) {
+          e0 = to_f<T>(qp[d]);
+          e1 = to_f<T>(qp[d + 1]);
+        }
+        w.q[n][t][y] = Pair<T>::pack(e0, e1);
+      }
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w.o[n][t][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w.m[n][e] = -INFINITY;
+      w.l[n][e] = 0.f;
+    }
+  }
+  int first = 0, count = 0;
+  if (a.shared)
+    count = (int)a.cache.fixed;
+  else
+    visible(a.cache, b, first, count);
+  const int per = (count + a.nsplit - 1) / a.nsplit;
+  const int lo = min(split * per, count), hi = min(lo + per, count);
+  w.template run<C>(a.cache, a.shared ? 0 : b, hk, first, lo, hi, wk, nk, a.scale_log2);
+  // O, m and l of the warp's rows to shared memory; lane (r, c) holds queries 2c, 2c + 1
+  float* mine = sm + warp * R * RS;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float l = w.l[n][e];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      float* row = mine + (8 * n + 2 * w.c + e) * RS;
+      if (w.r == 0) {
+        row[D] = w.m[n][e];
+        row[D + 1] = l;
+      }
+#pragma unroll
+      for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          constexpr int CV = Layout<C, D>::CV;
+          const int nt = 2 * t + h;
+          row[(nt / CV) * 8 * CV + w.r * CV + nt % CV] = w.o[n][t][2 * h + e];
+        }
+    }
+  __syncthreads();
+  // join the warps that split the keys, in their order
+  const int rows = min(a.warps_row * R, a.rows - tile * a.warps_row * R);
+  for (int i = threadIdx.x; i < rows * D; i += kThreads) {
+    const int lr = i / D, e = i - lr * D;
+    const float* p = sm + ((lr / R) * R + lr % R) * RS;  // warps 0 .. warps_row - 1 are the first key part
+    const int step = a.warps_row * R * RS;
+    float mx = p[D];
+    for (int x = 1; x < nk; ++x) mx = fmaxf(mx, p[x * step + D]);
+    const float use = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f, den = 0.f;
+    for (int x = 0; x < nk; ++x) {
+      const float f = ex2(p[x * step + D] - use);
+      sum += f * p[x * step + e];
+      den += f * p[x * step + D + 1];
+    }
+    int bb, h;
+    place(tile * a.warps_row * R + lr, bb, h);
+    const int64_t row = (int64_t)bb * a.Hq + h;
+    if (a.splits == 1) {
+      ((T*)a.out)[row * D + e] = from_f<T>(den == 0.f ? 0.f : sum / den);
+      if (e == 0 && a.lse) a.lse[row] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
+    } else {
+      float* dst = a.part + (row * a.splits + a.split0 + split) * (D + 2);
+      dst[e] = sum;
+      if (e == 0) {
+        dst[D] = mx;
+        dst[D + 1] = den;
+      }
+    }
+  }
+}
+
+template <typename T, typename C, int D, int NQ>
+void launch_mma(const MmaArgs& a, int Hkv, int B) {
+  const size_t smem = (size_t)kWarps * 8 * NQ * (D + 3) * sizeof(float);
+  if (smem > 48 * 1024)
+    C10_CUDA_CHECK(cudaFuncSetAttribute(decode_mma_kernel<T, C, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)smem));
+  decode_mma_kernel<T, C, D, NQ><<<dim3((unsigned)(a.nsplit * a.tiles), (unsigned)Hkv, (unsigned)(a.shared ? 1 : B)), kThreads,
+                                   smem, stream()>>>(a);
+}
+
+// 8, 16 or 32 query rows a warp
+template <typename T, typename C, int D>
+void launch_rows(MmaArgs& a, int Hkv, int B) {
+  if (a.rows <= 8) {
+    a.warps_row = 1;
+    a.tiles = 1;
+    launch_mma<T, C, D, 1>(a, Hkv, B);
+  } else if (!a.shared) {
+    a.warps_row = 1;
+    a.tiles = (a.rows + 15) / 16;
+    launch_mma<T, C, D, 2>(a, Hkv, B);
+  } else {
+    a.warps_row = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
+    a.tiles = (a.rows + 16 * a.warps_row - 1) / (16 * a.warps_row);
+    launch_mma<T, C, D, 2>(a, Hkv, B);
+  }
+}
+
+template <typename T, typename C>
+void launch_dim(MmaArgs& a, int Hkv, int B, int d) {
+  if (d == 64)
+    launch_rows<T, C, 64>(a, Hkv, B);
+  else if (d == 96)
+    launch_rows<T, C, 96>(a, Hkv, B);
+  else
+    launch_rows<T, C, 128>(a, Hkv, B);
+}
+
+bool mma_dim(int64_t d) { return d == 64 || d == 96 || d == 128; }
+
+// 16-byte rows, which the tensor-core path loads
+bool rows16(const CacheView& v, int64_t size) {
+  return (uintptr_t)v.data % 16 == 0 && v.sb * size % 16 == 0 && v.sh * size % 16 == 0 && v.ss * size % 16 == 0;
+}
+
+template <typename T>
+void launch_kind(MmaArgs& a, int kind, int Hkv, int B, int d) {
+  if (kind == KV_I8)
+    launch_dim<T, int8_t>(a, Hkv, B, d);
+  else if (kind == KV_E4M3)
+    launch_dim<T, e4m3>(a, Hkv, B, d);
+  else
+    launch_dim<T, T>(a, Hkv, B, d);
+}
+
 template <typename C, int LANES>
 void launch_simt(const DecodeArgs& a) {
   const int G = a.group == 1 ? 1 : 4;
@@ -342,12 +817,40 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
   a.group = (int)(Hq / Hkv);
   a.d = (int)d;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
-  const int64_t blocks = B * Hkv;
-  const int cs = pieces(std::min<int64_t>(S, window), blocks);
-  const int ps = has_prefix ? pieces(P, blocks) : 0;
+  const int kind = cache_kind(ck.scalar_type(), what);
+  const bool half_q = a.q_type != KV_F32;
+  const bool eight = kind == KV_I8 || kind == KV_E4M3;
+  const bool mma_cache = half_q && mma_dim(d) && (eight || kind == a.q_type) && rows16(a.src.k, ck.element_size()) &&
+                         rows16(a.src.v, ck.element_size());
+  const bool mma_prefix = half_q && mma_dim(d) && has_prefix;
+  const int cs = pieces(std::min<int64_t>(S, window), B * Hkv);
+  // the prefix is read once for the batch by the tensor-core path, once per sequence by the other
+  const int64_t prefix_rows = B * a.group, prefix_tile = prefix_rows <= 8 ? 8 : prefix_rows <= 16 ? 16 : prefix_rows <= 32 ? 32 : 64;
+  const int ps = !has_prefix ? 0 : pieces(P, mma_prefix ? Hkv * ((prefix_rows + prefix_tile - 1) / prefix_tile) : B * Hkv);
   a.splits = cs + ps;
-  at::Tensor part = at::empty({B * Hq, a.splits, d + 2}, q.options().dtype(at::kFloat));
-  a.part = part.data_ptr<float>();
+  at::Tensor part;
+  if (a.splits > 1 || !mma_cache) {
+    part = at::empty({B * Hq, a.splits, d + 2}, q.options().dtype(at::kFloat));
+    a.part = part.data_ptr<float>();
+  }
+  MmaArgs m{};
+  m.q = a.q;
+  m.sqb = a.sqb;
+  m.sqh = a.sqh;
+  m.part = a.part;
+  m.out = out.data_ptr();
+  m.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  m.splits = a.splits;
+  m.Hq = a.Hq;
+  m.group = a.group;
+  m.scale_log2 = a.scale_log2;
+  auto run_mma = [&](int k) {
+    if (a.q_type == KV_BF16)
+      launch_kind<__nv_bfloat16>(m, k, a.Hkv, a.B, a.d);
+    else
+      launch_kind<__half>(m, k, a.Hkv, a.B, a.d);
+    check_launch(what);
+  };
   if (has_prefix) {
     DecodeArgs p = a;
     p.src.k = prefix_view(*pk, hold_pk);
@@ -357,13 +860,32 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
     p.src.S = 1 << 30;
     p.nsplit = ps;
     p.split0 = 0;
-    launch_source(p, a.q_type);
-    check_launch(what);
+    if (mma_prefix) {
+      m.cache = p.src;
+      m.rows = (int)prefix_rows;
+      m.shared = true;
+      m.split0 = 0;
+      m.nsplit = ps;
+      run_mma(a.q_type);
+    } else {
+      launch_source(p, a.q_type);
+      check_launch(what);
+    }
   }
   a.nsplit = cs;
   a.split0 = ps;
-  launch_source(a, cache_kind(ck.scalar_type(), what));
-  check_launch(what);
+  if (mma_cache) {
+    m.cache = a.src;
+    m.rows = a.group;
+    m.shared = false;
+    m.split0 = ps;
+    m.nsplit = cs;
+    run_mma(kind);
+    if (a.splits == 1) return {out, lse};
+  } else {
+    launch_source(a, kind);
+    check_launch(what);
+  }
   const int64_t rows = B * Hq;
   TB_DISPATCH_FLOAT(q.scalar_type(), what, [&] {
     decode_join_kernel<scalar_t><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, stream()>>>(
