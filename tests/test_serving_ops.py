@@ -484,8 +484,8 @@ def test_attention_refusals():
 def _attention_bound(q, cache, lengths, pk, pv, window, scale, ref):
     """|error| of an output element.  Scores: d fp32 products and sums of |q||k| (2^-24 each, twice: products may be
     split between units) and the exponential's 2^-22, relative to the weight; weights rounded to the type of the
-    values' product (half a step each) times sum p|v| / sum p; the result rounded once.  The 8-bit kinds use bf16
-    weights whatever the queries' type."""
+    values' product (half a step each) times sum p|v| / sum p; the result rounded once.  The 8-bit kinds use fp16
+    weights whatever the queries' type, and fp16 queries (relative to the row's largest element: 2^-24 of it)."""
     d = q.shape[-1]
     mag = ops.KVCache(cache.k, cache.v.float().abs().to(cache.v.dtype), cache.k_scale,
                       None if cache.v_scale is None else cache.v_scale)
@@ -495,7 +495,8 @@ def _attention_bound(q, cache, lengths, pk, pv, window, scale, ref):
     if pk is not None and pk.numel():
         kmax = torch.maximum(kmax, pk.float().abs().amax())
     scores = 2 * d * 2.0 ** -24 * float(q.double().abs().sum(-1).max() * kmax) * scale + 2.0 ** -20
-    weight = 0.0 if q.dtype == torch.float32 else (HALF[torch.bfloat16] if cache.k_scale is not None else HALF[q.dtype])
+    # (a prefix beside an 8-bit cache is in the queries' type)
+    weight = 0.0 if q.dtype == torch.float32 else (HALF[torch.float16] if cache.k_scale is not None and pk is None else HALF[q.dtype])
     return (2 * scores + weight) * a + HALF[q.dtype] * 1.01 * ref.abs() + 2.0 ** -24, scores
 
 

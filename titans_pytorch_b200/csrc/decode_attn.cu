@@ -222,34 +222,52 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(DecodeArgs a) {
   }
 }
 
-// Joins the pieces of each row: one warp a row, split order.
+// Joins the pieces of each row, in a fixed order: one block a row, warp w takes
+// pieces w, w + 8, ... (one warp walking all pieces took 0.5 us a piece).
+constexpr int kJoinWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const float* __restrict__ part, int splits, int d,
-                                                               int64_t rows, T* __restrict__ out,
-                                                               float* __restrict__ lse) {
-  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const float* __restrict__ part, int splits, int d,
+                                                                      T* __restrict__ out, float* __restrict__ lse) {
+  __shared__ float sm_o[kJoinWarps][256], sm_l[kJoinWarps], sm_m[kJoinWarps];
+  const int64_t row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* p = part + row * splits * (d + 2);
   float m = -INFINITY;
-  for (int s = lane; s < splits; s += 32) m = fmaxf(m, p[(int64_t)s * (d + 2) + d]);
+  for (int s = threadIdx.x; s < splits; s += 32 * kJoinWarps) m = fmaxf(m, p[(int64_t)s * (d + 2) + d]);
   m = warp_max(m);
+  if (lane == 0) sm_m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm_m[w]);
   const float use = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int s = 0; s < splits; ++s) {
+  float o[8], l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] = 0.f;
+#pragma unroll 4
+  for (int s = warp; s < splits; s += kJoinWarps) {
     const float* ps = p + (int64_t)s * (d + 2);
-    l += exp2f(ps[d] - use) * ps[d + 1];
+    const float f = exp2f(ps[d] - use);
+    l += f * ps[d + 1];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (lane + 32 * k < d) o[k] += f * ps[lane + 32 * k];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int e = lane; e < d; e += 32) {
-    float o = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float* ps = p + (int64_t)s * (d + 2);
-      o += exp2f(ps[d] - use) * ps[e];
-    }
-    out[row * d + e] = from_f<T>(o * inv);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (lane + 32 * k < d) sm_o[warp][lane + 32 * k] = o[k];
+  if (lane == 0) sm_l[warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) l += sm_l[w];
+  const int e = threadIdx.x;
+  if (e < d) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) sum += sm_o[w][e];
+    out[row * d + e] = from_f<T>(l == 0.f ? 0.f : sum / l);
   }
-  if (lse && lane == 0) lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  if (lse && e == 0) lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------- tensor cores
@@ -273,8 +291,8 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const float* __re
 //
 // The running maximum moves only when a score exceeds it by more than 8 (in
 // log2): weights stay below 2^8, and most steps need no exchange between lanes.
-// 8-bit values are exact in bf16; their scale is multiplied into the weight, in
-// bf16 for its range.  Weights are rounded to 16 bits for the product (half a
+// 8-bit keys and values are exact in fp16; a value's scale is multiplied into its
+// weight.  Weights are rounded to 16 bits for the product (half a
 // step each); sums of them are taken before that, in fp32.
 
 template <typename T> struct Pair;  // two packed 16-bit floats
@@ -316,32 +334,39 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Bytes 0 and 2 of p as two numbers of the cache's type, in T, exactly.
-template <typename C, typename T> __device__ __forceinline__ uint32_t widen(uint32_t p);
-// int8 in bf16: 128 + (b & 127) less 128 + (b & 128)
-template <> __device__ __forceinline__ uint32_t widen<int8_t, __nv_bfloat16>(uint32_t p) {
-  const uint32_t x = (p & 0x007f007fu) | 0x43004300u, y = (p & 0x00800080u) | 0x43004300u;
-  __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-// int8 in fp16: 1024 + (b + 128) less 1152
-template <> __device__ __forceinline__ uint32_t widen<int8_t, __half>(uint32_t p) {
-  const uint32_t x = ((p & 0x00ff00ffu) ^ 0x00800080u) | 0x64006400u, y = 0x64806480u;
-  __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-// e4m3 in bf16: the same bits four places down are the number times 2^-120
-template <> __device__ __forceinline__ uint32_t widen<e4m3, __nv_bfloat16>(uint32_t p) {
-  const uint32_t x = ((p & 0x00800080u) << 8) | ((p & 0x007f007fu) << 4), y = 0x7b807b80u;
-  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-// e4m3 in fp16: one place down from the high byte, times 2^8
-template <> __device__ __forceinline__ uint32_t widen<e4m3, __half>(uint32_t p) {
-  const uint32_t x = ((p & 0x00800080u) << 8) | ((p & 0x007f007fu) << 7), y = 0x5c005c00u;
-  __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
+// 8-bit numbers widened to fp16, exactly.  The ALU pipe is what limits the 8-bit
+// kinds (half the issue rate), so these are counted in its operations.
+template <typename C> struct Widen;
+template <> struct Widen<int8_t> {
+  // bytes 0 and 2 of p: 1024 + (b + 128) less 1152
+  static __device__ __forceinline__ uint32_t even(uint32_t p) {
+    const uint32_t x = (p & 0x00ff00ffu) ^ 0x64806480u, y = 0x64806480u;
+    __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+  // a key's four bytes as two pairs: (0, 2) and (1, 3)
+  static __device__ __forceinline__ void key(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = even(w);
+    b = even(w >> 8);
+  }
+  // byte e of two values
+  static __device__ __forceinline__ uint32_t values(uint32_t v0, uint32_t v1, int e) {
+    return even(__byte_perm(v0, v1, e | ((4 + e) << 8)));
+  }
+};
+template <> struct Widen<e4m3> {
+  static __device__ __forceinline__ uint32_t two(uint32_t p) {  // bytes 0 and 1
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(p & 0xffffu), __NV_E4M3);
+    return (uint32_t)r.x | ((uint32_t)r.y << 16);
+  }
+  static __device__ __forceinline__ void key(uint32_t w, uint32_t& a, uint32_t& b) {  // pairs (0, 1) and (2, 3)
+    a = two(w);
+    b = two(w >> 16);
+  }
+  static __device__ __forceinline__ uint32_t values(uint32_t v0, uint32_t v1, int e) {
+    return two(__byte_perm(v0, v1, e | ((4 + e) << 4)));
+  }
+};
 
 template <typename C, int D> struct Layout {
   static constexpr bool k16 = sizeof(C) == 2;
@@ -349,6 +374,10 @@ template <typename C, int D> struct Layout {
   static constexpr int CV = k16 ? (D % 64 == 0 ? 8 : 4) : D == 128 ? 16 : D == 64 ? 8 : 4;  // of a value
   static constexpr int KW = D / 4 * sizeof(C) / 4;                     // words of a key a lane holds
   static constexpr int VW = D / 8 * sizeof(C) / 4;                     // words of a value (may end mid-word at D = 96)
+  // the dimension, of the four of a step, that is element y of pair x
+  static __device__ __forceinline__ int at(int x, int y) {
+    return std::is_same<C, int8_t>::value ? x + 2 * y : 2 * x + y;
+  }
   static constexpr int U = D == 64 ? (k16 ? 2 : 4) : k16 ? 1 : 2;       // groups of 16 keys a step
 };
 
@@ -372,38 +401,60 @@ struct MmaArgs {
   void* out;       // written directly when a row has one piece in all
   float* lse;
   int splits, split0, nsplit;
+  int piece;                   // keys of a piece
   int Hq, group, rows, tiles;  // query rows of a key head in this launch; tiles of them
   int warps_row;               // warps side by side over rows; the others split the keys
   bool shared;                 // rows run over the whole batch (prefix alone)
   float scale_log2;
 };
 
-template <typename T, int D, int NQ>
+// TM: the type of the products, fp16 beside 8-bit keys, else the queries'.
+template <typename TM, int D, int NQ>
 struct Warp {
   static constexpr int STEPS = D / 16, R = 8 * NQ;
   uint32_t q[NQ][STEPS][2];
   float o[NQ][STEPS][4];  // [dimension tile][d r / r + 8, query 2c / 2c + 1]
-  float m[NQ][2], l[NQ][2];
+  float m[NQ][2], l[NQ][2], scale[NQ][2];
   int r, c;
 
   // One kind of keys [lo, hi), every stride-th block of 16 U starting at `block`.
-  template <typename C>
-  __device__ __forceinline__ void run(const KeySource& s, int b, int hk, int first, int lo, int hi, int block, int stride,
-                                      float scale) {
+  // PLAIN: rows (and scales) one after the other and no wrap in the range, so
+  // that a whole step's addresses are constants away from two pointers.
+  template <typename C, bool PLAIN>
+  __device__ __forceinline__ void run(const KeySource& s, int b, int hk, int first, int lo, int hi, int block, int stride) {
     using L = Layout<C, D>;
-    using TV = typename std::conditional<L::k16, T, __nv_bfloat16>::type;
+    constexpr bool k8 = CacheTraits<C>::scaled;
     constexpr int U = NQ == 1 ? L::U : 1, KEYS = 16 * U;
     constexpr int NK = L::KW * 4 / (L::CK * (int)sizeof(C)), NV = D / (8 * L::CV);  // pieces
     constexpr int KB = L::CK * sizeof(C), VB = L::CV * sizeof(C), VWP = VB / 4;
     const C* kb = (const C*)s.k.data + b * s.k.sb + hk * s.k.sh + c * L::CK;
     const C* vb = (const C*)s.v.data + b * s.v.sb + hk * s.v.sh + r * L::CV;
+    const float* ksb = k8 ? s.k.scale + b * s.k.qb + hk * s.k.qh : nullptr;
+    const float* vsb = k8 ? s.v.scale + b * s.v.qb + hk * s.v.qh : nullptr;
     uint32_t kw[U][2][L::KW], vw[U][4][NV * VWP];
     float ks[U][2], vs[U][2];
-    auto slot_of = [&](int i) {
-      int x = first + i;
+    auto slot_of = [&](int i) -> int64_t {
+      const int x = first + i;
       return x >= s.S ? x - s.S : x;
     };
-    auto load_k = [&](int base) {
+    auto load_k = [&](int base, bool whole) {
+      if (PLAIN && whole) {
+        const C* p = kb + (int64_t)(first + base + r) * D;
+        const float* ps = k8 ? ksb + first + base + r : nullptr;
+        const float* pv = k8 ? vsb + first + base + r : nullptr;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < NK; ++j) load_words<KB>(p + (16 * u + 8 * h) * D + j * 4 * L::CK, &kw[u][h][j * (KB / 4)]);
+            if constexpr (k8) {
+              ks[u][h] = ps[16 * u + 8 * h];
+              vs[u][h] = pv[16 * u + 8 * h];
+            }
+          }
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -414,21 +465,35 @@ struct Warp {
             const C* p = kb + slot * s.k.ss;
 #pragma unroll
             for (int j = 0; j < NK; ++j) load_words<KB>(p + j * 4 * L::CK, &kw[u][h][j * (KB / 4)]);
-            if constexpr (CacheTraits<C>::scaled) {
-              ks[u][h] = s.k.scale[b * s.k.qb + hk * s.k.qh + slot * s.k.qs];
-              vs[u][h] = s.v.scale[b * s.v.qb + hk * s.v.qh + slot * s.v.qs];
+            if constexpr (k8) {
+              ks[u][h] = ksb[slot * s.k.qs];
+              vs[u][h] = vsb[slot * s.v.qs];
             }
+          } else if constexpr (k8) {
+            ks[u][h] = 0.f;
+            vs[u][h] = 0.f;
           }
         }
     };
-    auto load_v = [&](int base) {
+    auto load_v = [&](int base, bool whole) {
+      if (PLAIN && whole) {
+        const C* p = vb + (int64_t)(first + base + 2 * c) * D;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+              load_words<VB>(p + (16 * u + (x & 1) + 8 * (x >> 1)) * D + j * 8 * L::CV, &vw[u][x][j * VWP]);
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = base + 16 * u + 2 * c + (x & 1) + 8 * (x >> 1);
           if (i < hi) {
-            const C* p = vb + (int64_t)slot_of(i) * s.v.ss;
+            const C* p = vb + slot_of(i) * s.v.ss;
 #pragma unroll
             for (int j = 0; j < NV; ++j) load_words<VB>(p + j * 8 * L::CV, &vw[u][x][j * VWP]);
           } else {  // a weight of zero times whatever the slot holds has to be zero
@@ -439,8 +504,9 @@ struct Warp {
     };
     int base = lo + block * KEYS;
     if (base >= hi) return;
-    load_k(base);
-    load_v(base);
+    bool whole = base + KEYS <= hi;
+    load_k(base, whole);
+    load_v(base, whole);
     while (true) {
       float sc[U][NQ][4];
 #pragma unroll
@@ -456,43 +522,62 @@ struct Warp {
           uint32_t f[2][2];  // [key half][pair]
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if constexpr (L::k16) {
+            if constexpr (k8) {
+              Widen<C>::key(kw[u][h][t], f[h][0], f[h][1]);
+            } else {
               f[h][0] = kw[u][h][2 * t];
               f[h][1] = kw[u][h][2 * t + 1];
-            } else {
-              const uint32_t w = kw[u][h][t];
-              f[h][0] = widen<C, T>(__byte_perm(w, 0u, 0x4140));
-              f[h][1] = widen<C, T>(__byte_perm(w, 0u, 0x4342));
             }
           }
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) Pair<T>::mma(sc[u][n], f[0][0], f[1][0], f[0][1], f[1][1], q[n][t][0], q[n][t][1]);
+          for (int n = 0; n < NQ; ++n) Pair<TM>::mma(sc[u][n], f[0][0], f[1][0], f[0][1], f[1][1], q[n][t][0], q[n][t][1]);
         }
-      float vscale[U][2];
-      float grow = -INFINITY;
+      // the 8-bit kinds watch score + log2(value scale), so that the weights times that scale fit fp16
+      float vscale[U][2], grow = -INFINITY, lift[U][2];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const bool in = base + 16 * u + 8 * h + r < hi;
-          float f = scale;
-          if constexpr (CacheTraits<C>::scaled) {
-            f *= ks[u][h];
-            vscale[u][h] = in ? vs[u][h] : 0.f;
+          lift[u][h] = 0.f;
+          if constexpr (k8) {
+            vscale[u][h] = vs[u][h];
+            lift[u][h] = __log2f(vs[u][h]);  // -inf behind the end
           }
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float& x = sc[u][n][2 * h + e];
-              x = in ? x * f : -INFINITY;
-              grow = fmaxf(grow, x - m[n][e]);
+              x *= k8 ? ks[u][h] * scale[n][e] : scale[n][e];
             }
         }
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (base + 16 * u + 8 * h + r >= hi)
+#pragma unroll
+              for (int n = 0; n < NQ; ++n) {
+                sc[u][n][2 * h] = -INFINITY;
+                sc[u][n][2 * h + 1] = -INFINITY;
+              }
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mx = fmaxf(mx, k8 ? sc[u][n][2 * h + e] + lift[u][h] : sc[u][n][2 * h + e]);
+          // m = -inf at first: -inf - -inf is NaN and does not count, a finite score does
+          grow = fmaxf(grow, mx - m[n][e]);
+        }
       const int next = base + stride * KEYS;
-      const bool more = next < hi;
-      if (more) load_k(next);
-      // m = -inf at first: -inf - -inf is NaN and does not count, a finite score does
+      const bool more = next < hi, next_whole = next + KEYS <= hi;
+      if (more) load_k(next, next_whole);
       if (__any_sync(0xffffffffu, grow > 8.f)) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -500,7 +585,9 @@ struct Warp {
           for (int e = 0; e < 2; ++e) {
             float mx = m[n][e];
 #pragma unroll
-            for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(sc[u][n][e], sc[u][n][2 + e]));
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) mx = fmaxf(mx, k8 ? sc[u][n][2 * h + e] + lift[u][h] : sc[u][n][2 * h + e]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
             const float corr = mx == m[n][e] ? 1.f : ex2(m[n][e] - mx);
@@ -513,6 +600,11 @@ struct Warp {
             }
           }
       }
+      float use[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) use[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         uint32_t p[NQ][2];
@@ -523,11 +615,11 @@ struct Warp {
             float w[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              w[e] = ex2(sc[u][n][2 * h + e] - (m[n][e] == -INFINITY ? 0.f : m[n][e]));
+              w[e] = ex2(sc[u][n][2 * h + e] - use[n][e]);
               l[n][e] += w[e];
-              if constexpr (CacheTraits<C>::scaled) w[e] *= vscale[u][h];
+              if constexpr (k8) w[e] *= vscale[u][h];
             }
-            p[n][h] = transpose8x8(Pair<TV>::pack(w[0], w[1]));
+            p[n][h] = transpose8x8(Pair<TM>::pack(w[0], w[1]));
           }
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
@@ -537,31 +629,31 @@ struct Warp {
             const int nt = 2 * t + h, e = nt % L::CV, j = nt / L::CV;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              if constexpr (L::k16) {
+              if constexpr (k8) {
+                const int w = j * VWP + e / 4;
+                f[h][y] = Widen<C>::values(vw[u][2 * y][w], vw[u][2 * y + 1][w], e & 3);
+              } else {
                 const int w = j * VWP + e / 2;
                 f[h][y] = __byte_perm(vw[u][2 * y][w], vw[u][2 * y + 1][w], e & 1 ? 0x7632 : 0x5410);
-              } else {
-                const int w = j * VWP + e / 4;
-                // byte e of the two keys to bytes 0 and 2
-                f[h][y] = widen<C, TV>(
-                    __byte_perm(vw[u][2 * y][w], vw[u][2 * y + 1][w], 0x0000 | (e & 3) | ((4 + (e & 3)) << 8)));
               }
             }
           }
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) Pair<TV>::mma(o[n][t], f[0][0], f[1][0], f[0][1], f[1][1], p[n][0], p[n][1]);
+          for (int n = 0; n < NQ; ++n) Pair<TM>::mma(o[n][t], f[0][0], f[1][0], f[0][1], f[1][1], p[n][0], p[n][1]);
         }
       }
       if (!more) break;
-      load_v(next);
+      load_v(next, next_whole);
       base = next;
+      whole = next_whole;
     }
   }
 };
 
 template <typename T, typename C, int D, int NQ>
 __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(MmaArgs a) {
-  using W = Warp<T, D, NQ>;
+  using TM = typename std::conditional<CacheTraits<C>::scaled, __half, T>::type;
+  using W = Warp<TM, D, NQ>;
   constexpr int R = W::R, STEPS = W::STEPS;
   extern __shared__ float sm[];  // [warp][R][D + 2]: O, m, l (row stride odd against bank conflicts of the transposed store)
   constexpr int RS = D + 3;
@@ -585,19 +677,37 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
     if (row < a.rows) place(row, bb, h);
     const T* qp = (const T*)a.q + bb * a.sqb + h * a.sqh;
     // in the order of the dimensions that the keys' pieces have
+    float qf[STEPS][2][2], top = 0.f;
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        constexpr int CK = Layout<C, D>::CK;
-        const int d = (t / (CK / 4)) * 4 * CK + w.c * CK + (t % (CK / 4)) * 4 + 2 * y;
-        float e0 = 0.f, e1 = 0.f;
-        if (row < a.rows) {
-          e0 = to_f<T>(qp[d]);
-          e1 = to_f<T>(qp[d + 1]);
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          using L = Layout<C, D>;
+          constexpr int CK = L::CK;
+          const int d = (t / (CK / 4)) * 4 * CK + w.c * CK + (t % (CK / 4)) * 4 + L::at(x, y);
+          qf[t][x][y] = row < a.rows ? to_f<T>(qp[d]) : 0.f;
+          top = fmaxf(top, fabsf(qf[t][x][y]));
         }
-        w.q[n][t][y] = Pair<T>::pack(e0, e1);
+    // beside 8-bit keys: to fp16 by a power of two that brings the row's largest to [1, 2)
+    float down = 1.f, up = 1.f;
+    if constexpr (CacheTraits<C>::scaled) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = (__float_as_int(top) >> 23) - 127;
+      if (e > -100 && e < 100) {
+        down = __int_as_float((127 - e) << 23);
+        up = __int_as_float((127 + e) << 23);
       }
+    }
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) w.q[n][t][x] = Pair<TM>::pack(qf[t][x][0] * down, qf[t][x][1] * down);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)  // row 2c + e of the scores' layout
+      w.scale[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * w.c + e) * 4);
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
 #pragma unroll
@@ -613,9 +723,14 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
     count = (int)a.cache.fixed;
   else
     visible(a.cache, b, first, count);
-  const int per = (count + a.nsplit - 1) / a.nsplit;
-  const int lo = min(split * per, count), hi = min(lo + per, count);
-  w.template run<C>(a.cache, a.shared ? 0 : b, hk, first, lo, hi, wk, nk, a.scale_log2);
+  const int lo = min(split * a.piece, count), hi = min(lo + a.piece, count);
+  const KeySource& src = a.cache;
+  const bool plain = src.k.ss == D && src.v.ss == D && first + hi <= src.S &&
+                     (!CacheTraits<C>::scaled || (src.k.qs == 1 && src.v.qs == 1));
+  if (plain)
+    w.template run<C, true>(src, a.shared ? 0 : b, hk, first, lo, hi, wk, nk);
+  else
+    w.template run<C, false>(src, a.shared ? 0 : b, hk, first, lo, hi, wk, nk);
   // O, m and l of the warp's rows to shared memory; lane (r, c) holds queries 2c, 2c + 1
   float* mine = sm + warp * R * RS;
 #pragma unroll
@@ -748,11 +863,12 @@ void launch_source(const DecodeArgs& a, int kind) {
   });
 }
 
-// Pieces for `keys` keys a row: enough blocks for two rounds of the GPU, no
-// piece shorter than 128 keys.
+// Pieces for `keys` keys a row: enough blocks for two rounds of the GPU, pieces
+// of 128 to 1024 keys.  (The upper bound is for batches of unequal lengths: the
+// longest sequence's blocks must not be the last ones running.)
 int pieces(int64_t keys, int64_t blocks) {
   const int64_t want = (2 * 4 * num_sms() + blocks - 1) / blocks;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (keys + 127) / 128, 64}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(want, (keys + 1023) / 1024), (keys + 127) / 128));
 }
 
 // The prefix [P, Hkv, d] as a key source; `hold` keeps the copy that unaligned rows need.
@@ -866,6 +982,7 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
       m.shared = true;
       m.split0 = 0;
       m.nsplit = ps;
+      m.piece = (int)((P + ps - 1) / ps);
       run_mma(a.q_type);
     } else {
       launch_source(p, a.q_type);
@@ -880,6 +997,7 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
     m.shared = false;
     m.split0 = ps;
     m.nsplit = cs;
+    m.piece = (int)((std::min<int64_t>(S, window) + cs - 1) / cs);
     run_mma(kind);
     if (a.splits == 1) return {out, lse};
   } else {
@@ -887,9 +1005,10 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
     check_launch(what);
   }
   const int64_t rows = B * Hq;
+  TORCH_CHECK(rows < (1ll << 31), what, ": too many query rows in one call");
   TB_DISPATCH_FLOAT(q.scalar_type(), what, [&] {
-    decode_join_kernel<scalar_t><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, stream()>>>(
-        a.part, a.splits, (int)d, rows, (scalar_t*)out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr);
+    decode_join_kernel<scalar_t><<<(unsigned)rows, 32 * kJoinWarps, 0, stream()>>>(
+        a.part, a.splits, (int)d, (scalar_t*)out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr);
   });
   check_launch(what);
   return {out, lse};
