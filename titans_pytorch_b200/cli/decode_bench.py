@@ -59,6 +59,8 @@ def main(argv=None) -> None:
     ap.add_argument("--new", type=int, default=32)
     ap.add_argument("--which", default="recurrence,streaming,streaming_int8")
     ap.add_argument("--no-graph", action="store_true", help="streaming decoders: eager steps (no CUDA graph)")
+    ap.add_argument("--kv-cache", default=None, choices=["float32", "bfloat16", "float16", "int8", "fp8"],
+                    help="streaming decoders: type of the key/value ring, read by the fused attention")
     a = ap.parse_args(argv)
     torch.manual_seed(0)
     cfg = TitansConfig(vocab_size=a.vocab, dim=a.dim, num_layers=a.layers, num_heads=a.heads,
@@ -83,7 +85,7 @@ def main(argv=None) -> None:
                 generate(model, ids, a.new, greedy=True, states=st)
                 e.record()
             else:
-                dec = StreamingDecoder(model, batch=a.batch, graph=not a.no_graph)
+                dec = StreamingDecoder(model, batch=a.batch, graph=not a.no_graph, kv_cache=a.kv_cache)
                 dec.prefill(ids)
                 dec.step(nxt[:, :1])  # warm-up
                 torch.cuda.synchronize()

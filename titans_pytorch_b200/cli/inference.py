@@ -25,6 +25,8 @@ def build_parser() -> argparse.ArgumentParser:
     a("--temperature", type=float, default=1.0)
     a("--top-k", type=int, default=50)
     a("--top-p", type=float, default=0.9)
+    a("--min-p", type=float, default=0.0, help="keep tokens of at least this share of the likeliest one's probability")
+    a("--fused-sampling", action="store_true", help="sample with one kernel instead of sort + multinomial")
     a("--repetition-penalty", type=float, default=1.0)
     a("--interactive", action="store_true")
     a("--stream", action="store_true")
@@ -32,6 +34,8 @@ def build_parser() -> argparse.ArgumentParser:
     a("--decoder", choices=["recurrence", "incremental"], default="recurrence",
       help="recurrence: re-run the last chunk per token (the reference's decoding); incremental: one "
            "token per step over a sliding-window KV cache with the memory state carried (MAG / MAL / LMM)")
+    a("--kv-cache", choices=["float32", "bfloat16", "float16", "int8", "fp8"], default=None,
+      help="type of the incremental decoder's key/value ring, read by the fused attention (default: fp32, unfused)")
     a("--device", default=None)
     a("--seed", type=int, default=0)
     return p
@@ -42,16 +46,19 @@ def run_prompt(model, tok, prompt: str, args, out=sys.stdout) -> str:
     ids = tok.encode(prompt or " ", add_special_tokens=False) if hasattr(tok, "encode") else tok(prompt)
     x = torch.tensor([ids], dtype=torch.long, device=dev)
     kw = dict(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-              repetition_penalty=args.repetition_penalty, eos_token_id=getattr(tok, "eos_token_id", None))
+              repetition_penalty=args.repetition_penalty, eos_token_id=getattr(tok, "eos_token_id", None),
+              min_p=getattr(args, "min_p", 0.0), fused_sampling=getattr(args, "fused_sampling", False))
     if getattr(args, "decoder", "recurrence") == "incremental" and getattr(model, "model_type", "") != "mac":
         from ..inference.decode import generate_incremental
 
-        ids_, _ = generate_incremental(model, x, args.max_tokens, **kw)
+        ids_, _ = generate_incremental(model, x, args.max_tokens, kv_cache=getattr(args, "kv_cache", None), **kw)
         text = tok.decode(ids_[0, x.shape[1]:].tolist())
         out.write(prompt + text + "\n")
         return text
     if getattr(args, "decoder", "recurrence") == "incremental":
         print("note: MAC decodes with the recurrence (no incremental decoder for it)", file=sys.stderr)
+    if getattr(args, "kv_cache", None):
+        print("note: --kv-cache applies to --decoder incremental only", file=sys.stderr)
     if args.stream:
         text, n0 = "", x.shape[1]
         for ids_, _ in generate(model, x, args.max_tokens, stream=True, **kw):

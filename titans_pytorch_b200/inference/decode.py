@@ -27,6 +27,13 @@ Until the first update this equals a full forward over the stream's prefix
 (per-token logits of ``model(ids[:, :t+1])``), and the state after the first
 ``update_every`` tokens equals ``model(ids[:, :update_every])``'s new state;
 the tests check both, and the ring's wrap-around past ``window`` tokens.
+
+The ring is fp32 by default.  ``kv_cache="bfloat16" | "float16" | "int8" | "fp8"``
+keeps it in that type instead (half, or a quarter and a scale per token and
+head, of the bytes each step reads): a token is rotated, quantised and stored
+by one kernel (:func:`~titans_pytorch_b200.ops.kv_cache.kv_cache_write`) and the
+step's attention is :func:`~titans_pytorch_b200.ops.decode_attention.decode_attention`,
+which reads the persistent tokens once for the whole batch.
 """
 
 from __future__ import annotations
@@ -36,6 +43,8 @@ import torch
 from ..models.memory import MemoryState
 from ..ops.attention import rope_angles
 from ..ops.conv import conv_silu_norm_reference
+from ..ops.decode_attention import decode_attention
+from ..ops.kv_cache import KINDS, KVCache, kv_cache_write
 from ..ops.linear import linear
 from ..ops.memory import activation
 
@@ -57,7 +66,8 @@ class _LayerCache:
     memory inputs of the current update interval, and the memory state (all
     updated in place, so a captured step replays on the same buffers)."""
 
-    def __init__(self, block, batch: int, window: int, interval: int, device, dtype, state) -> None:
+    def __init__(self, block, batch: int, window: int, interval: int, device, dtype, state,
+                 kv_cache: str | None = None) -> None:
         self.block = block
         att = getattr(block, "attention", None)
         self.att = att
@@ -66,8 +76,11 @@ class _LayerCache:
         self.P = 0
         if att is not None:
             H, d = att.num_heads, att.head_dim
-            self.k = torch.zeros(batch, window, H, d, dtype=torch.float32, device=device)
-            self.v = torch.zeros(batch, window, H, d, dtype=torch.float32, device=device)
+            if kv_cache is None:
+                self.k = torch.zeros(batch, window, H, d, dtype=torch.float32, device=device)
+                self.v = torch.zeros(batch, window, H, d, dtype=torch.float32, device=device)
+            else:
+                self.cache = KVCache.allocate(batch, H, window, d, kv_cache, device)
             pers = block.persistent(1)
             P = pers.shape[1] if pers is not None else 0
             self.P = P
@@ -75,8 +88,14 @@ class _LayerCache:
                 pkv = att._project(pers[:1], kv_only=True)
                 pk = pkv[..., :D].reshape(1, P, H, d)
                 pv = pkv[..., D:].reshape(1, P, H, d).float()
-                if att.rope is not None:
+                if kv_cache is not None:  # [P, H, d], shared by the batch
+                    if att.rope is not None:
+                        pk = att.rope.rotate(pk, torch.arange(P, device=device), att.use_kernels)
+                    self.prefix_k, self.prefix_v = pk[0].contiguous(), pv[0].to(pk.dtype).contiguous()
+                    pk = pv = None
+                elif att.rope is not None:
                     pk = _rotate(pk, torch.arange(P, device=device), att.rope.inv_freq)
+            if P and kv_cache is None:
                 self.pk = pk.float().expand(batch, -1, -1, -1).contiguous()
                 self.pv = pv.expand(batch, -1, -1, -1).contiguous()
         ks = mem.config.conv_kernel_size if mem.use_conv else 1
@@ -93,11 +112,14 @@ class StreamingDecoder:
     memory states (one :class:`MemoryState` per block).  ``graph=True``
     (CUDA) captures the per-token step once and replays it (the step is a few
     hundred small launches); the memory update between intervals runs
-    eagerly and writes the states in place."""
+    eagerly and writes the states in place.  ``kv_cache`` (see the module
+    docstring): the ring's type, ``None`` for fp32 through PyTorch operations."""
 
     def __init__(self, model, batch: int = 1, window: int | None = None, update_every: int | None = None,
-                 states=None, graph: bool = False) -> None:
+                 states=None, graph: bool = False, kv_cache: str | None = None) -> None:
         cfg = model.config
+        if kv_cache is not None and kv_cache not in KINDS:
+            raise ValueError(f"kv_cache must be one of {tuple(KINDS)} or None, not {kv_cache!r}")
         if getattr(model, "model_type", "") == "mac":
             raise NotImplementedError("incremental decoding covers MAG, MAL and LMM; MAC attends over memory "
                                       "tokens retrieved for the whole segment (use generate())")
@@ -112,11 +134,14 @@ class StreamingDecoder:
         self.batch = batch
         sts = states if states is not None else [None] * len(model.blocks)
         with torch.no_grad():
-            self.layers = [_LayerCache(b, batch, self.window, self.update_every, self.device, self.dtype, st)
+            self.layers = [_LayerCache(b, batch, self.window, self.update_every, self.device, self.dtype, st, kv_cache)
                            for b, st in zip(model.blocks, sts, strict=True)]
         self.t = 0                                                          # host copy
         self.t_dev = torch.zeros(1, dtype=torch.long, device=self.device)   # the step's position
         self.ring_pos = torch.arange(self.window, device=self.device)
+        self.kv_cache = kv_cache
+        self.starts = self.t_dev.expand(batch)        # every sequence's position, for the cache operators
+        self.lengths = torch.ones(batch, dtype=torch.long, device=self.device)  # tokens written, the step's included
         self.graph = bool(graph) and self.device.type == "cuda"
         self._graph = None
         self._tok = torch.zeros(batch, 1, dtype=torch.long, device=self.device)
@@ -133,6 +158,13 @@ class StreamingDecoder:
         H, d = att.num_heads, att.head_dim
         D = H * d
         qkv = att._project(n)  # [B, 1, 3D]
+        if self.kv_cache is not None:
+            q, k, v = (qkv[..., i * D:(i + 1) * D].unflatten(-1, (H, d)) for i in range(3))
+            q = kv_cache_write(lc.cache, k, v, self.starts, q=q, rope_offset=lc.P, use_kernels=att.use_kernels,
+                               inv_freq=None if att.rope is None else att.rope.inv_freq)
+            o = decode_attention(q[:, 0], lc.cache, self.lengths, getattr(lc, "prefix_k", None),
+                                 getattr(lc, "prefix_v", None), scale=att.scale, use_kernels=att.use_kernels)
+            return linear(o.reshape(B, 1, D), att.proj_out.weight, use_kernels=att.use_kernels)
         q = qkv[..., :D].reshape(B, 1, H, d)
         k = qkv[..., D:2 * D].reshape(B, 1, H, d)
         v = qkv[..., 2 * D:].reshape(B, 1, H, d)
@@ -201,6 +233,7 @@ class StreamingDecoder:
             x = self._block(lc, x)
         logits = linear(model.norm(x), model.head.weight, use_kernels=model.config.use_kernels)[:, -1]
         self.t_dev += 1
+        self.lengths += 1
         return logits
 
     # ------------------------------------------------------------ API
@@ -254,16 +287,21 @@ def generate_incremental(model, input_ids: torch.Tensor, max_new_tokens: int = 1
                          top_k: int = 50, top_p: float = 0.9, repetition_penalty: float = 1.0,
                          eos_token_id: int | None = None, greedy: bool = False,
                          generator: torch.Generator | None = None, window: int | None = None,
-                         update_every: int | None = None):
-    """Generate with :class:`StreamingDecoder`; returns ``(ids, states)``."""
+                         update_every: int | None = None, kv_cache: str | None = None, min_p: float = 0.0,
+                         fused_sampling: bool = False):
+    """Generate with :class:`StreamingDecoder`; returns ``(ids, states)``.
+
+    ``kv_cache``: the ring's type; ``min_p``, ``fused_sampling``: see
+    :func:`~titans_pytorch_b200.inference.generate.sample_next`."""
     from .generate import sample_next
 
     dec = StreamingDecoder(model, batch=input_ids.shape[0], window=window, update_every=update_every,
-                           graph=input_ids.is_cuda)
+                           graph=input_ids.is_cuda, kv_cache=kv_cache)
     logits = dec.prefill(input_ids)
     generated = input_ids.to(dec.device).clone()
     for _ in range(max_new_tokens):
-        nxt = sample_next(logits.clone(), generated, temperature, top_k, top_p, repetition_penalty, greedy, generator)
+        nxt = sample_next(logits.clone(), generated, temperature, top_k, top_p, repetition_penalty, greedy, generator,
+                          min_p, fused_sampling)
         generated = torch.cat([generated, nxt.to(generated.dtype)], dim=1)
         if eos_token_id is not None and bool((nxt == eos_token_id).all()):
             break

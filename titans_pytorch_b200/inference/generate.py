@@ -23,6 +23,8 @@ from typing import Iterator
 import torch
 import torch.nn.functional as F
 
+from ..ops.sampling import sample_tokens
+
 
 # ----------------------------------------------------------------- sampling
 def apply_repetition_penalty(logits: torch.Tensor, generated: torch.Tensor, penalty: float) -> torch.Tensor:
@@ -52,8 +54,18 @@ def top_p_filter(logits: torch.Tensor, p: float) -> torch.Tensor:
 
 def sample_next(logits: torch.Tensor, generated: torch.Tensor, temperature: float = 1.0, top_k: int = 50,
                 top_p: float = 0.9, repetition_penalty: float = 1.0, greedy: bool = False,
-                generator: torch.Generator | None = None) -> torch.Tensor:
-    """Next token ids [B, 1] from last-position logits [B, V]."""
+                generator: torch.Generator | None = None, min_p: float = 0.0, fused: bool = False) -> torch.Tensor:
+    """Next token ids [B, 1] from last-position logits [B, V].
+
+    ``fused=True``, or ``min_p > 0``: one call of
+    :func:`~titans_pytorch_b200.ops.sampling.sample_tokens` with uniform numbers
+    from ``generator`` (other tokens than ``torch.multinomial`` would draw from
+    the same generator, of the same distribution)."""
+    if (fused or min_p > 0.0) and not greedy:
+        u = torch.rand(logits.shape[0], device=logits.device, generator=generator)
+        return sample_tokens(logits, u, temperature=max(temperature, 1e-7), top_k=top_k, top_p=min(max(top_p, 0.0), 1.0),
+                             min_p=min_p, generated=generated if repetition_penalty != 1.0 else None,
+                             repetition_penalty=repetition_penalty)[:, None]
     logits = logits.float() / max(temperature, 1e-7)
     logits = apply_repetition_penalty(logits, generated, repetition_penalty)
     if greedy:
@@ -72,15 +84,18 @@ def _context(model, generated: torch.Tensor, context_size: int | None) -> torch.
 def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 100, temperature: float = 1.0,
              top_k: int = 50, top_p: float = 0.9, repetition_penalty: float = 1.0,
              eos_token_id: int | None = None, states=None, stream: bool = False, greedy: bool = False,
-             context_size: int | None = None, generator: torch.Generator | None = None):
-    """Generate tokens; returns ``(ids, states)`` or, with ``stream=True``, an iterator of them."""
+             context_size: int | None = None, generator: torch.Generator | None = None, min_p: float = 0.0,
+             fused_sampling: bool = False):
+    """Generate tokens; returns ``(ids, states)`` or, with ``stream=True``, an iterator of them.
+
+    ``min_p``, ``fused_sampling``: see :func:`sample_next`."""
     def steps() -> Iterator:
         nonlocal states
         generated = input_ids.clone()
         for _ in range(max_new_tokens):
             logits, states = model(_context(model, generated, context_size), states=states)
             nxt = sample_next(logits[:, -1, :], generated, temperature, top_k, top_p, repetition_penalty,
-                              greedy, generator)
+                              greedy, generator, min_p, fused_sampling)
             generated = torch.cat([generated, nxt.to(generated.dtype)], dim=1)
             done = eos_token_id is not None and bool((nxt == eos_token_id).all())
             if stream:
@@ -241,12 +256,34 @@ class ContinuousBatcher:
         self._next_id = 0
 
     def add_request(self, input_ids: torch.Tensor, max_new_tokens: int = 50, temperature: float = 1.0,
-                    top_k: int = 50, top_p: float = 0.9, eos_token_id: int | None = None) -> int:
+                    top_k: int = 50, top_p: float = 0.9, eos_token_id: int | None = None, min_p: float = 0.0,
+                    seed: int | None = None) -> int:
+        """Queue a request; returns its id.  With a ``seed`` (or ``min_p``) its uniform numbers come from a
+        generator of its own, which nothing else served draws from, and all such requests of a step are
+        sampled by one :func:`~titans_pytorch_b200.ops.sampling.sample_tokens` call."""
+        uniform = None
+        if seed is not None or min_p > 0.0:
+            uniform = torch.Generator()
+            uniform.manual_seed(seed) if seed is not None else uniform.seed()
         rid = self._next_id
         self._next_id += 1
         self.queue.append(dict(id=rid, ids=input_ids.reshape(-1).to(self.device), left=max_new_tokens,
-                               temperature=temperature, top_k=top_k, top_p=top_p, eos=eos_token_id))
+                               temperature=temperature, top_k=top_k, top_p=top_p, eos=eos_token_id, min_p=min_p,
+                               uniform=uniform))
         return rid
+
+    def _sample_seeded(self, last: torch.Tensor) -> dict[int, torch.Tensor]:
+        """Next tokens of the active requests that have their own uniform numbers, in one call."""
+        rows = [i for i, r in enumerate(self.active) if r["uniform"] is not None]
+        if not rows:
+            return {}
+        rs = [self.active[i] for i in rows]
+        # one transfer: uniform numbers and settings, a row each
+        host = torch.tensor([[float(torch.rand((), generator=r["uniform"])), max(r["temperature"], 1e-7),
+                              r["top_p"], r["min_p"], float(r["top_k"])] for r in rs], dtype=torch.float32)
+        u, temp, p, m, k = host.to(last.device).unbind(1)
+        tok = sample_tokens(last[rows], u.contiguous(), temperature=temp, top_k=k, top_p=p, min_p=m)
+        return dict(zip(rows, tok))
 
     @torch.no_grad()
     def step(self) -> list[dict]:
@@ -263,8 +300,10 @@ class ContinuousBatcher:
         logits, _ = self.model(batch)
         last = logits[:, -1, :]
         finished, keep = [], []
+        seeded = self._sample_seeded(last)
         for i, r in enumerate(self.active):
-            nxt = sample_next(last[i:i + 1], r["ids"][None], r["temperature"], r["top_k"], r["top_p"])
+            nxt = seeded[i] if i in seeded else sample_next(last[i:i + 1], r["ids"][None], r["temperature"],
+                                                            r["top_k"], r["top_p"])
             r["ids"] = torch.cat([r["ids"], nxt.reshape(-1)])
             r["left"] -= 1
             if r["left"] <= 0 or (r["eos"] is not None and int(nxt) == r["eos"]):
