@@ -31,6 +31,7 @@ struct DecodeArgs {
   int q_type;
   int64_t sqb, sqh;
   float* part;        // [rows][splits][d + 2]: O, m, l
+  bool early;         // may start while the launch in front of it (the prefix) runs
   int splits, split0; // pieces a row has in all; the first of this launch
   int nsplit;         // pieces of this launch
   int B, Hq, Hkv, group, d;
@@ -85,6 +86,26 @@ template <typename C> struct Raw8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 
+// Launches of one call overlap: a kernel launched with `early` may start while
+// the one in front of it still runs, and waits for its results where it says so.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, bool early, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
 // fp32 arithmetic on the CUDA cores, any head dimension (a multiple of 8 up to
 // 256), any cache type.  LANES lanes share a key, 8 elements each; every group
 // of lanes keeps its own running (m, l, O) for G query heads of one key head.
@@ -93,6 +114,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(DecodeArgs a) {
   constexpr int KPW = 32 / LANES, GROUPS = KPW * kWarps, U = 4;
   __shared__ float sm_o[GROUPS][G][LANES * 8];
   __shared__ float sm_m[GROUPS][G], sm_l[GROUPS][G];
+  let_next_start();
   const int split = blockIdx.x % a.nsplit, gt = blockIdx.x / a.nsplit;
   const int hk = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -189,6 +211,8 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(DecodeArgs a) {
       }
     }
   }
+  // the kernel behind this one waits for this one alone: so this one ends after the one in front of it
+  wait_for_previous();
   const int grp = warp * KPW + sub;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -232,6 +256,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const floa
   const int64_t row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* p = part + row * splits * (d + 2);
+  wait_for_previous();
   float m = -INFINITY;
   for (int s = threadIdx.x; s < splits; s += 32 * kJoinWarps) m = fmaxf(m, p[(int64_t)s * (d + 2) + d]);
   m = warp_max(m);
@@ -395,6 +420,8 @@ template <int BYTES> __device__ __forceinline__ void load_words(const void* p, u
 
 struct MmaArgs {
   KeySource cache;
+  KeySource ahead;  // a short prefix, which the first piece sees in front of its cache keys (fixed = 0: none)
+  bool early;
   const void* q;
   int64_t sqb, sqh;
   float* part;
@@ -655,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
   using TM = typename std::conditional<CacheTraits<C>::scaled, __half, T>::type;
   using W = Warp<TM, D, NQ>;
   constexpr int R = W::R, STEPS = W::STEPS;
+  let_next_start();
   extern __shared__ float sm[];  // [warp][R][D + 2]: O, m, l (row stride odd against bank conflicts of the transposed store)
   constexpr int RS = D + 3;
   const int split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit;
@@ -724,6 +752,8 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
   else
     visible(a.cache, b, first, count);
   const int lo = min(split * a.piece, count), hi = min(lo + a.piece, count);
+  if constexpr (!CacheTraits<C>::scaled)
+    if (split == 0 && a.ahead.fixed > 0) w.template run<C, false>(a.ahead, 0, hk, 0, 0, (int)a.ahead.fixed, wk, nk);
   const KeySource& src = a.cache;
   const bool plain = src.k.ss == D && src.v.ss == D && first + hi <= src.S &&
                      (!CacheTraits<C>::scaled || (src.k.qs == 1 && src.v.qs == 1));
@@ -754,6 +784,8 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
           row[(nt / CV) * 8 * CV + w.r * CV + nt % CV] = w.o[n][t][2 * h + e];
         }
     }
+  // the kernel behind this one waits for this one alone: so this one ends after the one in front of it
+  wait_for_previous();
   __syncthreads();
   // join the warps that split the keys, in their order
   const int rows = min(a.warps_row * R, a.rows - tile * a.warps_row * R);
@@ -793,26 +825,215 @@ void launch_mma(const MmaArgs& a, int Hkv, int B) {
   if (smem > 48 * 1024)
     C10_CUDA_CHECK(cudaFuncSetAttribute(decode_mma_kernel<T, C, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)smem));
-  decode_mma_kernel<T, C, D, NQ><<<dim3((unsigned)(a.nsplit * a.tiles), (unsigned)Hkv, (unsigned)(a.shared ? 1 : B)), kThreads,
-                                   smem, stream()>>>(a);
+  launch(decode_mma_kernel<T, C, D, NQ>, dim3((unsigned)(a.nsplit * a.tiles), (unsigned)Hkv, (unsigned)(a.shared ? 1 : B)),
+         kThreads, smem, a.early, a);
 }
 
-// 8, 16 or 32 query rows a warp
+// The shared prefix against the queries of the whole batch: 64 or 128 rows a
+// block (16 or 32 a warp), so that each key is read from memory once per 128
+// rows.  Keys and values go through shared memory (cp.async, three tiles of 64
+// keys; rows padded by 16 bytes, which leaves ldmatrix free of bank conflicts),
+// as four warps share them; the products are as above.  With 128 rows the tensor
+// cores have work for about as long as memory; at mma.sync's rate that suffices.
+constexpr int kTile = 64, kStages = 3;
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&f)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&f)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+               : "r"(addr));
+}
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) decode_prefix_kernel(MmaArgs a) {
+  constexpr int STEPS = D / 16, R = 8 * NQ, ROW = D * 2 + 16, TILE = kTile * ROW;
+  let_next_start();
+  extern __shared__ __align__(16) uint8_t smem[];  // [stage][K, V][kTile][ROW]
+  const uint32_t sbase = (uint32_t)__cvta_generic_to_shared(smem);
+  const int split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit, hk = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int row0 = (tile * kWarps + warp) * R;
+  const int lo = split * a.piece, hi = min(lo + a.piece, (int)a.cache.fixed);
+  const int tiles = (hi - lo + kTile - 1) / kTile;
+  const T* kb = (const T*)a.cache.k.data + hk * a.cache.k.sh;
+  const T* vb = (const T*)a.cache.v.data + hk * a.cache.v.sh;
+  auto fetch = [&](int t) {
+    if (t < tiles) {
+      const uint32_t dst = sbase + (t % kStages) * 2 * TILE;
+      constexpr int CH = D / 8;  // 16-byte pieces of a row
+#pragma unroll
+      for (int i = threadIdx.x; i < kTile * CH; i += kThreads) {
+        const int key = i / CH, p = i - key * CH;
+        const int at = lo + t * kTile + key;
+        const int n = at < hi ? 16 : 0;  // zeros behind the end
+        const int64_t g = min(at, hi - 1);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst + key * ROW + p * 16),
+                     "l"(kb + g * a.cache.k.ss + p * 8), "r"(n)
+                     : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst + TILE + key * ROW + p * 16),
+                     "l"(vb + g * a.cache.v.ss + p * 8), "r"(n)
+                     : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < kStages - 1; ++t) fetch(t);
+  uint32_t q[NQ][STEPS][2];
+  float o[NQ][STEPS][4], m[NQ][2], l[NQ][2];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = row0 + 8 * n + r;
+    const int bb = row < a.rows ? row / a.group : 0, h = hk * a.group + (row < a.rows ? row - bb * a.group : 0);
+    const T* qp = (const T*)a.q + bb * a.sqb + h * a.sqh + 2 * c;
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float e0 = row < a.rows ? to_f<T>(qp[16 * t + 8 * x]) : 0.f;
+        const float e1 = row < a.rows ? to_f<T>(qp[16 * t + 8 * x + 1]) : 0.f;
+        q[n][t][x] = Pair<T>::pack(e0, e1);
+      }
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][t][e] = 0.f;
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+  }
+  const uint32_t k_lane = ((lane & 7) + ((lane >> 3) & 1) * 8) * ROW + (lane >> 4) * 16;
+  const uint32_t v_lane = ((lane & 7) + (lane >> 4) * 8) * ROW + ((lane >> 3) & 1) * 16;
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+    __syncthreads();  // the tile is here for every warp, and the one before it is done with
+    fetch(t + kStages - 1);
+    const uint32_t ks = sbase + (t % kStages) * 2 * TILE, vs = ks + TILE;
+    const int left = hi - lo - t * kTile;
+#pragma unroll
+    for (int g = 0; g < kTile / 16; ++g) {
+      if (g * 16 >= left) break;
+      float sc[NQ][4];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        uint32_t f[4];
+        ldmatrix4(f, ks + g * 16 * ROW + s * 32 + k_lane);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) Pair<T>::mma(sc[n], f[0], f[1], f[2], f[3], q[n][s][0], q[n][s][1]);
+      }
+      float grow = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[n][e] *= a.scale_log2;
+          if (left < kTile && g * 16 + (e >> 1) * 8 + r >= left) sc[n][e] = -INFINITY;
+          grow = fmaxf(grow, sc[n][e] - m[n][e & 1]);
+        }
+      if (__any_sync(0xffffffffu, grow > 8.f)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(m[n][e], fmaxf(sc[n][e], sc[n][2 + e]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float corr = mx == m[n][e] ? 1.f : ex2(m[n][e] - mx);
+            m[n][e] = mx;
+            l[n][e] *= corr;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+              o[n][s][e] *= corr;
+              o[n][s][2 + e] *= corr;
+            }
+          }
+      }
+      uint32_t p[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[e] = ex2(sc[n][2 * h + e] - (m[n][e] == -INFINITY ? 0.f : m[n][e]));
+            l[n][e] += w[e];
+          }
+          p[n][h] = transpose8x8(Pair<T>::pack(w[0], w[1]));
+        }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        uint32_t f[4];
+        ldmatrix4_trans(f, vs + g * 16 * ROW + s * 32 + v_lane);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) Pair<T>::mma(o[n][s], f[0], f[1], f[2], f[3], p[n][0], p[n][1]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+  wait_for_previous();
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sum = l[n][e];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      const int row = row0 + 8 * n + 2 * c + e;
+      if (row >= a.rows) continue;
+      const int bb = row / a.group, h = hk * a.group + row - bb * a.group;
+      float* dst = a.part + (((int64_t)bb * a.Hq + h) * a.splits + a.split0 + split) * (D + 2);
+      if (r == 0) {
+        dst[D] = m[n][e];
+        dst[D + 1] = sum;
+      }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        dst[16 * s + r] = o[n][s][e];
+        dst[16 * s + 8 + r] = o[n][s][2 + e];
+      }
+    }
+}
+
+// rows of a block of decode_prefix_kernel: 32 a warp where the accumulators fit the registers
+int prefix_block_rows(int64_t rows, int64_t d) { return rows > 64 && d == 64 ? 128 : 64; }
+
+template <typename T, int D, int NQ>
+void launch_prefix_rows(const MmaArgs& a, int Hkv) {
+  constexpr size_t smem = (size_t)kStages * 2 * kTile * (D * 2 + 16);
+  C10_CUDA_CHECK(cudaFuncSetAttribute(decode_prefix_kernel<T, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int tiles = (a.rows + kWarps * 8 * NQ - 1) / (kWarps * 8 * NQ);
+  launch(decode_prefix_kernel<T, D, NQ>, dim3((unsigned)(a.nsplit * tiles), (unsigned)Hkv), kThreads, smem, a.early, a);
+}
+template <typename T>
+void launch_prefix(const MmaArgs& a, int Hkv, int d) {
+  if (d == 64 && prefix_block_rows(a.rows, d) == 128)
+    launch_prefix_rows<T, 64, 4>(a, Hkv);
+  else if (d == 64)
+    launch_prefix_rows<T, 64, 2>(a, Hkv);
+  else if (d == 96)
+    launch_prefix_rows<T, 96, 2>(a, Hkv);
+  else
+    launch_prefix_rows<T, 128, 2>(a, Hkv);
+}
+
+// 8 or 16 query rows a warp
 template <typename T, typename C, int D>
 void launch_rows(MmaArgs& a, int Hkv, int B) {
-  if (a.rows <= 8) {
-    a.warps_row = 1;
-    a.tiles = 1;
+  a.warps_row = 1;
+  a.tiles = (a.rows + 15) / 16;
+  if (a.rows <= 8)
     launch_mma<T, C, D, 1>(a, Hkv, B);
-  } else if (!a.shared) {
-    a.warps_row = 1;
-    a.tiles = (a.rows + 15) / 16;
+  else
     launch_mma<T, C, D, 2>(a, Hkv, B);
-  } else {
-    a.warps_row = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
-    a.tiles = (a.rows + 16 * a.warps_row - 1) / (16 * a.warps_row);
-    launch_mma<T, C, D, 2>(a, Hkv, B);
-  }
 }
 
 template <typename T, typename C>
@@ -847,9 +1068,9 @@ void launch_simt(const DecodeArgs& a) {
   const int G = a.group == 1 ? 1 : 4;
   const dim3 grid((unsigned)(a.nsplit * ((a.group + G - 1) / G)), (unsigned)a.Hkv, (unsigned)a.B);
   if (G == 1)
-    decode_simt_kernel<C, LANES, 1><<<grid, kThreads, 0, stream()>>>(a);
+    launch(decode_simt_kernel<C, LANES, 1>, grid, kThreads, 0, a.early, a);
   else
-    decode_simt_kernel<C, LANES, 4><<<grid, kThreads, 0, stream()>>>(a);
+    launch(decode_simt_kernel<C, LANES, 4>, grid, kThreads, 0, a.early, a);
 }
 
 void launch_source(const DecodeArgs& a, int kind) {
@@ -938,11 +1159,20 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
   const bool eight = kind == KV_I8 || kind == KV_E4M3;
   const bool mma_cache = half_q && mma_dim(d) && (eight || kind == a.q_type) && rows16(a.src.k, ck.element_size()) &&
                          rows16(a.src.v, ck.element_size());
-  const bool mma_prefix = half_q && mma_dim(d) && has_prefix;
+  // A short prefix is seen by the cache's own kernel (16-bit kinds): one launch less.  A longer one is read once for
+  // the whole batch by the tensor-core path, once per sequence by the other.
+  const bool inline_prefix = has_prefix && mma_cache && !eight && P <= 128;
+  const bool mma_prefix = half_q && mma_dim(d) && has_prefix && !inline_prefix;
   const int cs = pieces(std::min<int64_t>(S, window), B * Hkv);
-  // the prefix is read once for the batch by the tensor-core path, once per sequence by the other
-  const int64_t prefix_rows = B * a.group, prefix_tile = prefix_rows <= 8 ? 8 : prefix_rows <= 16 ? 16 : prefix_rows <= 32 ? 32 : 64;
-  const int ps = !has_prefix ? 0 : pieces(P, mma_prefix ? Hkv * ((prefix_rows + prefix_tile - 1) / prefix_tile) : B * Hkv);
+  const int64_t prefix_rows = B * a.group;
+  const bool many_rows = mma_prefix && prefix_rows > 16;
+  int ps = 0;
+  if (has_prefix && !inline_prefix) {
+    const int64_t block_rows = many_rows ? prefix_block_rows(prefix_rows, d) : 16;
+    const int64_t blocks = mma_prefix ? Hkv * ((prefix_rows + block_rows - 1) / block_rows) : B * Hkv;
+    // many rows: a block a third of an SM, one round of the GPU, pieces of whole tiles
+    ps = many_rows ? (int)std::max<int64_t>(1, std::min<int64_t>(3 * num_sms() / blocks, (P + 255) / 256)) : pieces(P, blocks);
+  }
   a.splits = cs + ps;
   at::Tensor part;
   if (a.splits > 1 || !mma_cache) {
@@ -967,7 +1197,12 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
       launch_kind<__half>(m, k, a.Hkv, a.B, a.d);
     check_launch(what);
   };
-  if (has_prefix) {
+  if (inline_prefix) {
+    m.ahead.k = prefix_view(*pk, hold_pk);
+    m.ahead.v = prefix_view(*pv, hold_pv);
+    m.ahead.fixed = P;
+    m.ahead.S = 1 << 30;
+  } else if (has_prefix) {
     DecodeArgs p = a;
     p.src.k = prefix_view(*pk, hold_pk);
     p.src.v = prefix_view(*pv, hold_pv);
@@ -983,7 +1218,16 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
       m.split0 = 0;
       m.nsplit = ps;
       m.piece = (int)((P + ps - 1) / ps);
-      run_mma(a.q_type);
+      if (many_rows) {
+        m.piece = (m.piece + kTile - 1) / kTile * kTile;
+        if (a.q_type == KV_BF16)
+          launch_prefix<__nv_bfloat16>(m, a.Hkv, a.d);
+        else
+          launch_prefix<__half>(m, a.Hkv, a.d);
+        check_launch(what);
+      } else {
+        run_mma(a.q_type);
+      }
     } else {
       launch_source(p, a.q_type);
       check_launch(what);
@@ -991,6 +1235,7 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
   }
   a.nsplit = cs;
   a.split0 = ps;
+  a.early = m.early = ps > 0;
   if (mma_cache) {
     m.cache = a.src;
     m.rows = a.group;
@@ -1007,8 +1252,8 @@ std::vector<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& 
   const int64_t rows = B * Hq;
   TORCH_CHECK(rows < (1ll << 31), what, ": too many query rows in one call");
   TB_DISPATCH_FLOAT(q.scalar_type(), what, [&] {
-    decode_join_kernel<scalar_t><<<(unsigned)rows, 32 * kJoinWarps, 0, stream()>>>(
-        a.part, a.splits, (int)d, (scalar_t*)out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr);
+    launch(decode_join_kernel<scalar_t>, dim3((unsigned)rows), 32 * kJoinWarps, 0, true, a.part, a.splits, (int)d,
+           (scalar_t*)out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr);
   });
   check_launch(what);
   return {out, lse};
