@@ -36,74 +36,89 @@ struct WriteArgs {
   const float* freq;
   int64_t start_s, count_s, offset;
   int T, S, d, n;
+  int tokens;  // of a block
+  FastDiv by_token;  // rows of a token
   float amplitude;
   int half;
 };
 
-// 8 elements of row x from column c, rotated.  tab: cos / sin of the token's pairs.
+// 8 elements of row x from column c, rotated.  cs, sn: the token's tables,
+// padded with (1, 0) to a multiple of 8 pairs.
 template <typename T>
-__device__ __forceinline__ void rotated8(const T* x, int c, const float2* tab, int n, bool half, float (&v)[8]) {
+__device__ __forceinline__ void rotated8(const T* x, int c, const float* cs, const float* sn, int n, bool half, float (&v)[8]) {
   load8<T>(x + c, v);
   if (c >= 2 * n) return;
   if (!half) {
+    float a[4], b[4];
+    table_load(cs + c / 2, a);
+    table_load(sn + c / 2, b);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      const int p = (c + i) >> 1;
-      if (p < n) {
-        const float2 cs = tab[p];
-        const float a = v[i], b = v[i + 1];
-        v[i] = a * cs.x - b * cs.y;
-        v[i + 1] = a * cs.y + b * cs.x;
-      }
+      const float p = v[i], q = v[i + 1];
+      v[i] = p * a[i / 2] - q * b[i / 2];
+      v[i + 1] = p * b[i / 2] + q * a[i / 2];
     }
+  } else if (n % 8 == 0) {  // the partners are a vector of their own
+    const bool low = c < n;
+    const int at = low ? c : c - n;
+    float w[8], a[8], b[8];
+    load8<T>(x + (low ? c + n : c - n), w);
+    table_load(cs + at, a);
+    table_load(sn + at, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = low ? v[i] * a[i] - w[i] * b[i] : w[i] * b[i] + v[i] * a[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int j = c + i;
-      if (j < n) {
-        const float2 cs = tab[j];
-        v[i] = v[i] * cs.x - to_f<T>(x[j + n]) * cs.y;
-      } else if (j < 2 * n) {
-        const float2 cs = tab[j - n];
-        v[i] = to_f<T>(x[j - n]) * cs.y + v[i] * cs.x;
-      }
+      if (j < n)
+        v[i] = v[i] * cs[j] - to_f<T>(x[j + n]) * sn[j];
+      else if (j < 2 * n)
+        v[i] = to_f<T>(x[j - n]) * sn[j - n] + v[i] * cs[j - n];
     }
   }
 }
 
-// Block = one token of one sequence, all its heads: first the token's cos /
+// Block = a few tokens of one sequence, all their heads: first the tokens' cos /
 // sin, then LANES lanes per row (a power of two >= d / 8), 8 elements a lane.
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
-  extern __shared__ float2 tab[];  // [n]
-  const int t = blockIdx.x, b = blockIdx.y;
+  extern __shared__ __align__(16) float tab[];  // [token] cos, then sin of the pairs
+  const int np = (a.n + 7) & ~7;
+  const int t0 = blockIdx.x * a.tokens, b = blockIdx.y;
+  const int toks = min(a.tokens, a.T - t0);
   const int64_t start = a.start[b * a.start_s];
   int64_t count = a.count ? a.count[b * a.count_s] : a.T;
   count = min(max(count, (int64_t)0), (int64_t)a.T);
-  const int64_t pos = start + t;
   // a token that a later one of this call would overwrite is not stored, nor one before position 0
-  const bool stored = t < count && t >= count - a.S && pos >= 0;
-  if (!stored && a.q.p == nullptr) return;
-  for (int p = threadIdx.x; p < a.n; p += kThreads) tab[p] = rope_cos_sin(pos + a.offset, a.freq[p], a.amplitude);
+  auto stored = [&](int t) { return t < count && t >= count - a.S && start + t >= 0; };
+  for (int i = threadIdx.x; i < toks * np; i += kThreads) {
+    const int k = i / np, p = i - k * np;
+    const float2 cs = p < a.n ? rope_cos_sin(start + t0 + k + a.offset, a.freq[p], a.amplitude) : make_float2(1.f, 0.f);
+    tab[2 * k * np + p] = cs.x;
+    tab[(2 * k + 1) * np + p] = cs.y;
+  }
+  __shared__ int sh_slot;  // of the block's first token (where it has one): one 64-bit division a block
+  if (threadIdx.x == 0) sh_slot = (int)((start + t0) % a.S);
   __syncthreads();
-  const int slot = stored ? (int)(pos % a.S) : 0;
   const int lane = threadIdx.x % LANES;
   const int c = lane * 8;
   const bool on = c < a.d;
-  const int rows = a.q.H + (stored ? a.k.H + a.v.H : 0);
+  const int per_tok = a.q.H + a.k.H + a.v.H, rows = toks * per_tok;
   // whole warps stay in the loop for the shuffles
   for (int r0 = 0; r0 < rows; r0 += kThreads / LANES) {
-    const int r = r0 + threadIdx.x / LANES;
+    const int row = r0 + threadIdx.x / LANES;
+    int r;
+    const int k = a.by_token(row, r), t = t0 + k;
+    const float* cs = tab + 2 * k * np;
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (r < a.q.H) {
-      if (on) {
-        const T* src = (const T*)a.q.p + b * a.q.sb + t * a.q.st + r * a.q.sh;
-        rotated8<T>(src, c, tab, a.n, a.half, x);
-        store8<T>((T*)a.q_out + (((int64_t)b * a.T + t) * a.q.H + r) * a.d + c, x);
-      }
+    if (row < rows && r < a.q.H && on) {
+      const T* src = (const T*)a.q.p + b * a.q.sb + t * a.q.st + r * a.q.sh;
+      rotated8<T>(src, c, cs, cs + np, a.n, a.half, x);
+      store8<T>((T*)a.q_out + (((int64_t)b * a.T + t) * a.q.H + r) * a.d + c, x);
     }
     const int kv = r - a.q.H;
-    const bool mine = kv >= 0 && r < rows;
+    const bool mine = row < rows && kv >= 0 && stored(t);
     const bool is_v = kv >= a.k.H;
     const int h = is_v ? kv - a.k.H : kv;
     if (mine && on) {
@@ -112,31 +127,30 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
       if (is_v)
         load8<T>(src + c, x);
       else
-        rotated8<T>(src, c, tab, a.n, a.half, x);
+        rotated8<T>(src, c, cs, cs + np, a.n, a.half, x);
     }
+    // (positions of a block that begins before position 0 wrap here, not in C++'s remainder)
+    int64_t slot = sh_slot + k;
+    slot = slot < 0 ? slot + a.S : slot;
+    if (slot >= a.S) slot %= a.S;
     const CacheView& dst = is_v ? a.cv : a.ck;
+    if (!__any_sync(0xffffffffu, mine)) continue;  // queries only
     if constexpr (CacheTraits<C>::scaled) {
-      float amax = 0.f;
-      bool bad = false;
+      // the largest magnitude by its bits: infinities and NaN come out above every number
+      uint32_t top_bits = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        amax = fmaxf(amax, fabsf(x[i]));
-        bad |= !isfinite(x[i]);
-      }
-      int bad_any = bad;
+      for (int i = 0; i < 8; ++i) top_bits = max(top_bits, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        bad_any |= __shfl_xor_sync(0xffffffffu, bad_any, o);
-      }
+      for (int o = LANES / 2; o > 0; o >>= 1) top_bits = max(top_bits, __shfl_xor_sync(0xffffffffu, top_bits, o));
+      const float amax = __uint_as_float(top_bits);
       constexpr float top = CacheTraits<C>::top;
-      const bool full = amax >= 7.888609052210118e-31f && !bad_any;  // 2^-100
+      const bool bad = top_bits >= 0x7f800000u;
+      const bool full = amax >= 7.888609052210118e-31f && !bad;  // 2^-100
       const float inv = full ? top / amax : 0.f;
-      float scale = full ? amax / top : 1.f;
-      if (bad_any) scale = __int_as_float(0x7fffffff);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = bad_any ? 0.f : x[i] * inv;
-      if (mine && lane == 0) dst.scale[b * dst.qb + h * dst.qh + slot * dst.qs] = scale;
+      for (int i = 0; i < 8; ++i) x[i] = bad ? 0.f : x[i] * inv;
+      if (mine && lane == 0)
+        dst.scale[b * dst.qb + h * dst.qh + slot * dst.qs] = bad ? __int_as_float(0x7fffffff) : full ? amax / top : 1.f;
     }
     if (mine && on) store8<C>((C*)dst.data + b * dst.sb + h * dst.sh + slot * dst.ss + c, x);
   }
@@ -149,34 +163,50 @@ struct ReadArgs {
   const int64_t* lengths;
   int64_t len_s;
   int H, S, n, d;
+  FastDiv by_row;  // pieces of a row
 };
 
 // Row i of the output: the i-th of the newest min(length, slots, n) tokens, in
 // order; zeros behind the last.  Block = rows_per_block rows of one (sequence,
-// head, keys or values); one thread moves 8 elements.
+// head, keys or values); one thread moves four times 8 elements.
 template <typename C, typename T>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
-  const int per_row = a.d / 8;
-  const int64_t i64 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int h = blockIdx.y % a.H, b = blockIdx.y / a.H;
-  const int i = (int)(i64 / per_row), c = (int)(i64 - (int64_t)i * per_row) * 8;
-  if (i >= a.n) return;
   const bool is_v = blockIdx.z;
   const CacheView& src = is_v ? a.cv : a.ck;
   const int64_t len = max(a.lengths[b * a.len_s], (int64_t)0);
-  const int64_t held = min(len, (int64_t)min(a.S, a.n));
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (i < held) {
-    const int64_t slot = (len - held + i) % a.S;
-    load8<C>((const C*)src.data + b * src.sb + h * src.sh + slot * src.ss + c, x);
-    if constexpr (CacheTraits<C>::scaled) {
-      const float s = src.scale[b * src.qb + h * src.qh + slot * src.qs];
+  const int held = (int)min(len, (int64_t)min(a.S, a.n));
+  __shared__ int sh_first;  // the first token's slot: one 64-bit division a block
+  if (threadIdx.x == 0) sh_first = (int)((len - held) % a.S);
+  __syncthreads();
+  // four rows' pieces in flight a thread
+  constexpr int U = 4;
+  float x[U][8];
+  int at[U], col[U];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] *= s;
+  for (int u = 0; u < U; ++u) {
+    int c;
+    const int i = a.by_row((int)((blockIdx.x * U + u) * kThreads + threadIdx.x), c);
+    c *= 8;
+    at[u] = i;
+    col[u] = c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[u][k] = 0.f;
+    if (i < held) {
+      int64_t slot = sh_first + i;
+      if (slot >= a.S) slot -= a.S;
+      load8<C>((const C*)src.data + b * src.sb + h * src.sh + slot * src.ss + c, x[u]);
+      if constexpr (CacheTraits<C>::scaled) {
+        const float s = src.scale[b * src.qb + h * src.qh + slot * src.qs];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[u][k] *= s;
+      }
     }
   }
   T* dst = (T*)(is_v ? a.vo : a.ko);
-  store8<T>(dst + ((int64_t)blockIdx.y * a.n + i) * a.d + c, x);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (at[u] < a.n) store8<T>(dst + ((int64_t)blockIdx.y * a.n + at[u]) * a.d + col[u], x[u]);
 }
 
 // `hold` keeps the copy that unaligned rows need.
@@ -191,9 +221,12 @@ Rows rows_of(const at::Tensor& x, at::Tensor& hold, const char* what) {
 }
 
 template <typename T, typename C>
-void launch_write(const WriteArgs& a, int64_t B) {
-  const dim3 grid((unsigned)a.T, (unsigned)B);
-  const size_t smem = a.n * sizeof(float2);
+void launch_write(WriteArgs a, int64_t B) {
+  // several tokens a block, so that the table's latency is paid less often, while the GPU is full without it
+  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(8, B * a.T / (num_sms() * 4)));
+  a.by_token = FastDiv((uint32_t)(a.q.H + a.k.H + a.v.H));
+  const dim3 grid((unsigned)((a.T + a.tokens - 1) / a.tokens), (unsigned)B);
+  const size_t smem = (size_t)a.tokens * ((a.n + 7) & ~7) * 2 * sizeof(float);
   if (a.d <= 64)
     kv_write_kernel<T, C, 8><<<grid, kThreads, smem, stream()>>>(a);
   else if (a.d <= 128)
@@ -291,8 +324,10 @@ std::vector<at::Tensor> kv_cache_read(const at::Tensor& ck, const at::Tensor& cv
   a.S = (int)S;
   a.n = (int)n;
   a.d = (int)d;
+  a.by_row = FastDiv((uint32_t)(d / 8));
   const int64_t vecs = n * (d / 8);
-  const dim3 grid((unsigned)((vecs + kThreads - 1) / kThreads), (unsigned)(B * H), 2);
+  TORCH_CHECK(vecs < (1ll << 31) - 8 * kThreads, what, ": too many slots in one call");
+  const dim3 grid((unsigned)((vecs + 4 * kThreads - 1) / (4 * kThreads)), (unsigned)(B * H), 2);
   const int kind = cache_kind(ck.scalar_type(), what);
   TB_DISPATCH_FLOAT(dtype, what, [&] {
     TB_DISPATCH_CACHE(kind, what,

@@ -20,6 +20,7 @@ struct RopeArgs {
   int64_t tokens;  // B * T
   int T, H, d, n;
   float amplitude, sign;
+  FastDiv by_token, by_head, by_t, by_pair;  // work items of a token, of a head; T; pairs of a token
 };
 
 constexpr int kThreads = 256;
@@ -27,62 +28,96 @@ constexpr int kThreads = 256;
 // Interleaved: a 16-byte vector holds whole pairs; the table is padded with
 // (1, 0) past the rotated part, so the copied tail needs no branch.
 // Half: a work item is a pair of vectors (i, i + n) or one vector of the tail.
+//
+// The vectors are requested before the table is computed, so that the loads
+// and the fp64 angles wait at the same time (47 -> 38 us for 8 x 4096 x 24 x 64
+// bf16, against 31 us for the bytes alone).
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(kThreads) rope_vec_kernel(RopeArgs a, int tok_per_block) {
-  constexpr int V = Vec16<T>::N;
-  extern __shared__ float2 tab[];  // [tok_per_block][pairs]
+  constexpr int V = Vec16<T>::N, ITEMS = HALF ? 2 : 4;  // work items a thread has in flight
+  extern __shared__ __align__(16) float tab_raw[];         // cos [tok_per_block][pairs], then sin
+  float* tab = tab_raw;
   const int pairs = HALF ? a.n : a.d / 2;
-  const int64_t tok0 = (int64_t)blockIdx.x * tok_per_block;
+  const int tok0 = blockIdx.x * tok_per_block;
   const int toks = (int)min((int64_t)tok_per_block, a.tokens - tok0);
+  const int rot = a.n / V, head_items = HALF ? rot + (a.d - 2 * a.n) / V : a.d / V;
+  const int tok_items = a.H * head_items, items = toks * tok_items;
+  struct Item {
+    uint4 x, y;
+    T* dst;
+    int t, v;
+  } it[ITEMS];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      const int i = base + q * kThreads + threadIdx.x;
+      if (i < items) {
+        int rem, v, tt;
+        const int t = a.by_token(i, rem), h = a.by_head(rem, v);
+        const int tok = tok0 + t, b = a.by_t(tok, tt);
+        const T* x = (const T*)a.x + b * a.sxb + tt * a.sxt + h * a.sxh;
+        it[q].dst = (T*)a.y + ((int64_t)tok * a.H + h) * a.d;
+        it[q].t = t;
+        it[q].v = v;
+        const int at = HALF && v >= rot ? 2 * a.n + (v - rot) * V : v * V;
+        it[q].x = *reinterpret_cast<const uint4*>(x + at);
+        if (HALF && v < rot) it[q].y = *reinterpret_cast<const uint4*>(x + a.n + at);
+      }
+    }
+  };
+  fetch(0);
   for (int i = threadIdx.x; i < toks * pairs; i += kThreads) {
-    const int t = i / pairs, p = i - t * pairs;
-    const int tok = (int)tok0 + t;
-    const int b = tok / a.T, tt = tok - b * a.T;
+    int p, tt;
+    const int t = a.by_pair(i, p);
+    const int tok = tok0 + t, b = a.by_t(tok, tt);
     float2 cs = make_float2(1.f, 0.f);
     if (p < a.n) {
       cs = rope_cos_sin(a.pos[b * a.spb + tt * a.spt], a.freq[p], a.amplitude);
       cs.y *= a.sign;
     }
-    tab[i] = cs;
+    tab[i] = cs.x;
+    tab[tok_per_block * pairs + i] = cs.y;
   }
   __syncthreads();
-  const int head_items = HALF ? a.n / V + (a.d - 2 * a.n) / V : a.d / V;
-  const int tok_items = a.H * head_items;
-  for (int i = threadIdx.x; i < toks * tok_items; i += kThreads) {
-    const int t = i / tok_items, r = i - t * tok_items;
-    const int h = r / head_items, v = r - h * head_items;
-    const int tok = (int)tok0 + t;
-    const int b = tok / a.T, tt = tok - b * a.T;
-    const T* x = (const T*)a.x + b * a.sxb + tt * a.sxt + h * a.sxh;
-    T* y = (T*)a.y + ((int64_t)tok * a.H + h) * a.d;
-    const float2* cs = tab + t * pairs;
-    if constexpr (HALF) {
-      if (v < a.n / V) {
-        float p[V], q[V], u[V], w[V];
-        load16<T>(x + v * V, p);
-        load16<T>(x + a.n + v * V, q);
+  for (int base = 0; base < items; base += ITEMS * kThreads) {
+    if (base) fetch(base);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float2 c = cs[v * V + k];
-          u[k] = p[k] * c.x - q[k] * c.y;
-          w[k] = p[k] * c.y + q[k] * c.x;
+    for (int q = 0; q < ITEMS; ++q) {
+      if (base + q * kThreads + (int)threadIdx.x >= items) break;
+      const float* cs = tab + it[q].t * pairs;
+      const float* sn = cs + tok_per_block * pairs;
+      const int v = it[q].v;
+      Vec16<T> x, y;
+      x.raw = it[q].x;
+      if constexpr (HALF) {
+        if (v < rot) {
+          y.raw = it[q].y;
+          float u[V], w[V], c[V], n[V];
+          table_load(cs + v * V, c);
+          table_load(sn + v * V, n);
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float p0 = to_f<T>(x.v[k]), p1 = to_f<T>(y.v[k]);
+            u[k] = p0 * c[k] - p1 * n[k];
+            w[k] = p0 * n[k] + p1 * c[k];
+          }
+          store16<T>(it[q].dst + v * V, u);
+          store16<T>(it[q].dst + a.n + v * V, w);
+        } else {
+          *reinterpret_cast<uint4*>(it[q].dst + 2 * a.n + (v - rot) * V) = it[q].x;
         }
-        store16<T>(y + v * V, u);
-        store16<T>(y + a.n + v * V, w);
       } else {
-        const int at = 2 * a.n + (v - a.n / V) * V;
-        *reinterpret_cast<uint4*>(y + at) = *reinterpret_cast<const uint4*>(x + at);
-      }
-    } else {
-      float p[V], u[V];
-      load16<T>(x + v * V, p);
+        float u[V], c[V / 2], n[V / 2];
+        table_load(cs + v * (V / 2), c);
+        table_load(sn + v * (V / 2), n);
 #pragma unroll
-      for (int k = 0; k < V; k += 2) {
-        const float2 c = cs[(v * V + k) / 2];
-        u[k] = p[k] * c.x - p[k + 1] * c.y;
-        u[k + 1] = p[k] * c.y + p[k + 1] * c.x;
+        for (int k = 0; k < V; k += 2) {
+          const float p0 = to_f<T>(x.v[k]), p1 = to_f<T>(x.v[k + 1]);
+          u[k] = p0 * c[k / 2] - p1 * n[k / 2];
+          u[k + 1] = p0 * n[k / 2] + p1 * c[k / 2];
+        }
+        store16<T>(it[q].dst + v * V, u);
       }
-      store16<T>(y + v * V, u);
     }
   }
 }
@@ -90,7 +125,8 @@ __global__ void __launch_bounds__(kThreads) rope_vec_kernel(RopeArgs a, int tok_
 // Any size, stride and alignment: one element pair (or one tail element) per item.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rope_scalar_kernel(RopeArgs a, bool half, int64_t sxd) {
-  extern __shared__ float2 tab[];
+  extern __shared__ __align__(16) float tab_raw[];
+  float2* tab = reinterpret_cast<float2*>(tab_raw);
   const int tok = blockIdx.x;
   const int b = tok / a.T, tt = tok - b * a.T;
   for (int p = threadIdx.x; p < a.n; p += kThreads) {
@@ -162,11 +198,16 @@ at::Tensor rotary_embedding(const at::Tensor& x, const at::Tensor& pos, const at
                                                                                                 x.stride(3));
       return;
     }
-    // enough tokens a block for about four vectors a thread, if that still fills the GPU
-    const int64_t items = H * d / V;
-    int64_t per = std::max<int64_t>(1, 4 * kThreads / items);
+    // enough tokens a block for four rounds of its loads, if that still fills the GPU: the table's latency
+    // is paid once a block
+    const int64_t items = half ? H * (n / V + (d - 2 * n) / V) : H * d / V;
+    int64_t per = std::max<int64_t>(1, 4 * (half ? 2 : 4) * kThreads / std::max<int64_t>(items, 1));
     per = std::min(per, std::max<int64_t>(1, a.tokens / (num_sms() * 4)));
     per = std::min<int64_t>(per, 16);
+    a.by_token = FastDiv((uint32_t)std::max<int64_t>(items, 1));
+    a.by_head = FastDiv((uint32_t)std::max<int64_t>(items / H, 1));
+    a.by_t = FastDiv((uint32_t)T);
+    a.by_pair = FastDiv((uint32_t)std::max<int64_t>(half ? n : d / 2, 1));
     const size_t smem = per * (half ? std::max<int64_t>(n, 1) : d / 2) * sizeof(float2);
     const unsigned blocks = (unsigned)((a.tokens + per - 1) / per);
     if (half)

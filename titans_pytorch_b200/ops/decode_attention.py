@@ -77,14 +77,13 @@ def decode_attention(q: torch.Tensor, cache: KVCache, lengths: torch.Tensor, pre
     if window < 1:
         raise ValueError(f"window must be at least 1, not {window}")
     scale = d ** -0.5 if scale is None else float(scale)
-    q = q.detach()
     if want_kernels(q, use_kernels):
         if q.stride(-1) != 1:
             q = q.contiguous()
         out, lse = ext().decode_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lengths, prefix_k, prefix_v,
                                           window, scale, return_lse)
     else:
-        out, lse = decode_attention_reference(q, cache, lengths, prefix_k, prefix_v, window, scale)
+        out, lse = decode_attention_reference(q.detach(), cache, lengths, prefix_k, prefix_v, window, scale)
     return (out, lse) if return_lse else out
 
 

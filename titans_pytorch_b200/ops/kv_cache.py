@@ -115,11 +115,9 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: torc
     if inv_freq is not None and (inv_freq.dim() != 1 or 2 * inv_freq.numel() > d):
         raise ValueError(f"inv_freq must be [n] with 2n <= {d}, not {tuple(inv_freq.shape)}")
     if want_kernels(cache.k, use_kernels):
-        with torch.no_grad():
-            r = ext().kv_cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k.detach(), v.detach(), start,
-                                     counts, None if q is None else q.detach(),
-                                     None if inv_freq is None else inv_freq.float().contiguous(),
-                                     layout == "half", float(amplitude), int(rope_offset))
+        r = ext().kv_cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, start, counts, q,
+                                 None if inv_freq is None else inv_freq.float().contiguous(), layout == "half",
+                                 float(amplitude), int(rope_offset))
         return None if q is None else r
     return _write_reference(cache, k.detach(), v.detach(), start, counts, None if q is None else q.detach(), inv_freq,
                             layout, amplitude, rope_offset)
@@ -160,8 +158,7 @@ def kv_cache_read(cache: KVCache, lengths: torch.Tensor, n: int | None = None, d
     if not 0 <= n <= S:
         raise ValueError(f"n must be between 0 and the {S} slots, not {n}")
     if want_kernels(cache.k, use_kernels):
-        k, v = ext().kv_cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, lengths, n, dtype)
-        return k, v
+        return tuple(ext().kv_cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, lengths, n, dtype))
     held = lengths.clamp(0, min(S, n))[:, None]
     i = torch.arange(n, device=lengths.device)
     slot = ((lengths[:, None] - held + i) % S)[:, None, :]

@@ -112,7 +112,10 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     if inv_freq.dim() != 1 or 2 * inv_freq.numel() > x.shape[-1]:
         raise ValueError(f"inv_freq must be [n] with 2n <= {x.shape[-1]}, not {tuple(inv_freq.shape)}")
     if want_kernels(x, use_kernels):
-        return _RotaryFn.apply(x, positions, inv_freq.float().contiguous(), layout == "half", float(amplitude), False)
+        inv_freq = inv_freq.float().contiguous()
+        if x.requires_grad and torch.is_grad_enabled():
+            return _RotaryFn.apply(x, positions, inv_freq, layout == "half", float(amplitude), False)
+        return ext().rotary_embedding(x, positions, inv_freq, layout == "half", float(amplitude), False)
     return rotary_embedding_reference(x, positions, inv_freq, layout, amplitude)
 
 

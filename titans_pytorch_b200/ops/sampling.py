@@ -33,7 +33,7 @@ def _row(value, like: torch.Tensor, dtype: torch.dtype, name: str):
     if value.shape != like.shape[:1] or value.device != like.device:
         raise ValueError(f"{name} must be a number or [{like.shape[0]}] on the logits' device, "
                          f"not {tuple(value.shape)} on {value.device}")
-    return value.to(dtype).contiguous(), 0
+    return (value if value.dtype == dtype else value.to(dtype)).contiguous(), 0
 
 
 def sample_tokens_reference(logits, uniform, temperature, top_k, top_p, min_p, generated, repetition_penalty):
@@ -102,7 +102,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
         if generated is not None and generated.stride(1) != 1:
             generated = generated.contiguous()
         flat = [x for pair in rows for x in pair]
-        token, logprob = ext().sample_tokens(logits.detach(), uniform.contiguous(), *flat, generated)
+        token, logprob = ext().sample_tokens(logits, uniform.contiguous(), *flat, generated)
     else:
         full = [t if t is not None else torch.full((B,), s, dtype=d, device=logits.device)
                 for (t, s), d in zip(rows, (torch.float32, torch.int64) + (torch.float32,) * 3)]
