@@ -189,6 +189,21 @@ def test_rope_kernel_edges():
 
 
 @gpu
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_kernel_widest_heads(layout):
+    """Enough tokens of the widest head that a block's tables reach the limit of its shared memory."""
+    _cuda()
+    freq, _ = ops.rope_frequencies(1024, device="cuda")
+    x = torch.randn(1, 12000, 1, 1024, device="cuda", dtype=torch.bfloat16)
+    pos = torch.arange(12000, device="cuda")
+    y = ops.rotary_embedding(x, pos, freq, layout=layout)
+    ref = rotary_embedding_reference(x.double(), pos, freq, layout)
+    assert ((y.double() - ref).abs() <= _rope_bound(x, ref, torch.bfloat16, 1.0)).all()
+    with pytest.raises(RuntimeError):
+        ops.rotary_embedding(torch.zeros(1, 1, 1, 1032, device="cuda"), pos[:1], freq)
+
+
+@gpu
 def test_rope_double_backward_and_graph():
     _cuda()
     freq, _ = ops.rope_frequencies(32, device="cuda")
@@ -395,6 +410,9 @@ def test_cache_kernel_edges():
     ops.kv_cache_write(c, k, k, start, counts=start)
     ops.kv_cache_write(c, k, k, start - 100)
     assert torch.equal(c.k, before)
+    none = ops.KVCache.allocate(B, 0, S, d, "int8", device="cuda")
+    assert ops.kv_cache_write(none, k[:, :, :0], k[:, :, :0], start) is None
+    assert ops.kv_cache_read(none, start)[0].shape == (B, 0, S, d)
     # rows that are not aligned, and a layer of a stack whose neighbours stay as they were
     stack = [torch.zeros(3, B, H, S, d, dtype=torch.int8, device="cuda") for _ in range(2)]
     scales = [torch.ones(3, B, H, S, device="cuda") for _ in range(2)]

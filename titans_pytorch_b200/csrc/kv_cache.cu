@@ -293,7 +293,7 @@ at::Tensor kv_cache_write(at::Tensor& ck, at::Tensor& cv, const c10::optional<at
   a.T = (int)T;
   a.S = (int)ck.size(2);
   a.d = (int)d;
-  if (B == 0 || T == 0) return q_out;
+  if (B == 0 || T == 0 || a.q.H + 2 * H == 0) return q_out;
   const int kind = cache_kind(ck.scalar_type(), what);
   TB_DISPATCH_FLOAT(k.scalar_type(), what, [&] {
     TB_DISPATCH_CACHE(kind, what, [&] { launch_write<scalar_t, cache_t>(a, B); });

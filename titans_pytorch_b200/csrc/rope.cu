@@ -205,12 +205,13 @@ at::Tensor rotary_embedding(const at::Tensor& x, const at::Tensor& pos, const at
     const int64_t items = half ? H * (n / V + (d - 2 * n) / V) : H * d / V;
     int64_t per = std::max<int64_t>(1, 2 * (half ? 2 : 4) * kThreads / std::max<int64_t>(items, 1));
     per = std::min(per, std::max<int64_t>(1, a.tokens / (num_sms() * 4)));
-    per = std::min<int64_t>(per, 16);
+    const int64_t pair_bytes = (half ? std::max<int64_t>(n, 1) : d / 2) * sizeof(float2);
+    per = std::min<int64_t>({per, 16, 48 * 1024 / pair_bytes});
     a.by_token = FastDiv((uint32_t)std::max<int64_t>(items, 1));
     a.by_head = FastDiv((uint32_t)std::max<int64_t>(items / H, 1));
     a.by_t = FastDiv((uint32_t)T);
     a.by_pair = FastDiv((uint32_t)std::max<int64_t>(half ? n : d / 2, 1));
-    const size_t smem = per * (half ? std::max<int64_t>(n, 1) : d / 2) * sizeof(float2);
+    const size_t smem = per * pair_bytes;
     const unsigned blocks = (unsigned)((a.tokens + per - 1) / per);
     if (half)
       rope_vec_kernel<scalar_t, true><<<blocks, kThreads, smem, stream()>>>(a, (int)per);

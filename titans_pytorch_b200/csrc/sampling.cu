@@ -30,9 +30,9 @@
 //      passed over instead;
 //   4. the draw is the same search over the index: kept weight in 1024 index
 //      bins, then the elements of one bin.
-// Rows without top-k and top-p need 1 and 4 only, and so do rows where min-p
-// cuts above top-p's border for certain; after 3 the draw works on the list if
-// that holds everything that may be kept.
+// Rows without a filter need 1 and 4 only.  Where min-p cuts above top-p's
+// border for certain, which the counts tell, top-p is left out.  After 3 the draw
+// works on the list if that holds everything that may be kept.
 //
 // One block does all of this for a row; while SMs are free, up to seven more
 // take parts of the passes and add their counts, sums and list entries to its
@@ -53,6 +53,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kBins = kThreads;          // one a thread
 constexpr int kTable = 16;               // entries of the exponential's table
+constexpr int kShort = kThreads / 8;     // a list that is compared all against all
 constexpr int kSharedLimit = 226 * 1024;
 
 // one value for every row, or one per row
@@ -227,8 +228,7 @@ struct Row {
   // exp(z - zmax) * 2^F, as a double, by the table-driven method (Tang, 1989):
   // x = k ln2 / 16 + r, 2^(k / 16) from the table and the exponent, e^r by its
   // series to r^6 (|r| <= 0.022: 5e-16 beyond it).  Sixteen doubles fill the
-  // shared-memory banks once, so lanes never wait for one another (a table of
-  // 256 with a shorter series did: 20 against 9 us for a row of 32000).
+  // shared-memory banks once, so lanes never wait for one another.
   // Without branches, so that the chains of a vector's elements overlap.
   __device__ __forceinline__ double weight(uint32_t key) const {
     // the fp32 value as a double by its bits (a conversion takes eight times an
@@ -649,6 +649,52 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     }
     R.cluster_sync(blocks);
     if (rank > 0 && route == LIST_ALL) return;  // the rest is the first block's alone
+    if (route == LIST_ALL && s.list_n <= kShort) {
+      // A short list: every element against every other, eight lanes an element,
+      // gives its rank and the weight in front of it, by value and then by index,
+      // with two barriers instead of a search each.
+      const int n = s.list_n, i = tid >> 3, part = tid & 7;
+      u64* ms = reinterpret_cast<u64*>(s.n);
+      const uint2 e = i < n ? list[i] : make_uint2(0u, 0u);
+      const double w = R.weight(e.x);
+      const u64 m = i < n ? R.fixed(w) : 0ull;
+      if (i < n && part == 0) ms[i] = m;
+      __syncthreads();
+      int above = 0;
+      u64 front = 0ull;
+      if (i < n)
+        for (int j = part; j < n; j += 8) {
+          const uint2 f = list[j];
+          above += f.x > e.x;
+          front += f.x > e.x || (f.x == e.x && f.y < e.y) ? ms[j] : 0ull;
+        }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        above += __shfl_xor_sync(0xffffffffu, above, o);
+        front += __shfl_xor_sync(0xffffffffu, front, o);
+      }
+      bool in = i < n && (!by_count || above < want_k);
+      if (by_mass) {
+        if (by_count) total = R.block_sum(in && part == 0 ? m : 0ull);
+        in = in && front <= (u64)floor(fmax(p, 0.0) * (double)total);
+      }
+      const u64 mine = in && w >= least ? m : 0ull;
+      const u64 all = R.block_sum(part == 0 ? mine : 0ull);  // (and every thread has read ms)
+      if (i < n && part == 0) ms[i] = mine;
+      __syncthreads();
+      const u64 goal = min((u64)floor(fmax(u, 0.0) * (double)all), all - 1ull);
+      u64 run = 0ull;
+      if (i < n)
+        for (int j = part; j < n; j += 8) run += list[j].y < e.y ? ms[j] : 0ull;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+      if (part == 0 && mine && run <= goal && goal < run + mine) {
+        a.token[row] = (int64_t)e.y;
+        a.logprob[row] =
+            (float)((e.x == R.top_key ? 0.0 : (double)value_of(e.x) - R.zmax) - log((double)all / s.table[0]));
+      }
+      return;
+    }
     if (rank == 0) {
       R.listed = route == LIST_ALL || route == LIST_BORDER;
       if (by_count) {
