@@ -166,10 +166,10 @@ struct Row {
       groups_of<true>(i0, i1, f);
   }
   template <bool SCALE, typename F> __device__ __forceinline__ void groups_of(int i0, int i1, F f) const {
-    // Four vectors in flight a thread, each register reloaded as soon as it is
+    // Two vectors in flight a thread, each register reloaded as soon as it is
     // used (moving them along would wait for the loads).  Whole blocks of
     // vectors first, so that the loop over them checks nothing.
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 2;
     int rest = i0;
     if (vec) {
       const int v0 = i0 / VEC + threadIdx.x;  // i0 is a multiple of VEC
