@@ -1084,12 +1084,12 @@ void launch_source(const DecodeArgs& a, int kind) {
   });
 }
 
-// Pieces for `keys` keys a row: enough blocks for two rounds of the GPU, pieces
+// Pieces for `keys` keys a row: one round of the GPU at three blocks an SM, pieces
 // of 128 to 1024 keys.  (The upper bound is for batches of unequal lengths: the
 // longest sequence's blocks must not be the last ones running.)
 int pieces(int64_t keys, int64_t blocks) {
   if (keys <= 512) return 1;  // joining pieces of less costs more than it saves
-  const int64_t want = (2 * 4 * num_sms() + blocks - 1) / blocks;
+  const int64_t want = 3 * num_sms() / blocks;
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(want, (keys + 1023) / 1024), (keys + 127) / 128));
 }
 
