@@ -835,6 +835,21 @@ def test_sampling_kernel_ties_and_masks(fill):
 
 
 @gpu
+@pytest.mark.parametrize("B", [1, 40, 160])
+@pytest.mark.parametrize("fill", ["equal", "two", "flat"])
+def test_sampling_kernel_borders_longer_than_the_list(fill, B):
+    """Borders among more elements than the candidate list holds, with one block and with several a row."""
+    _cuda()
+    V = 131072
+    g = _gen(31, "cuda")
+    x = torch.randn(B, V, generator=g, device="cuda")
+    x = torch.full_like(x, -3.5) if fill == "equal" else (x > 0.5).float() if fill == "two" else x / 64
+    u = torch.rand(B, generator=g, device="cuda")
+    for kw in (dict(top_p=0.5), dict(top_k=100000), dict(top_k=90000, top_p=0.6), dict(min_p=0.5), dict(top_p=0.7, min_p=0.9)):
+        _check_sampling(x, u, **kw)
+
+
+@gpu
 def test_sampling_kernel_special_rows_and_graph():
     _cuda()
     _special_rows("cuda")
