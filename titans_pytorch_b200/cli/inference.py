@@ -41,7 +41,8 @@ def build_parser() -> argparse.ArgumentParser:
     return p
 
 
-def run_prompt(model, tok, prompt: str, args, out=sys.stdout) -> str:
+def run_prompt(model, tok, prompt: str, args, out=None) -> str:
+    out = sys.stdout if out is None else out  # at the call: stdout may be another one than at import
     dev = next(model.parameters()).device
     ids = tok.encode(prompt or " ", add_special_tokens=False) if hasattr(tok, "encode") else tok(prompt)
     x = torch.tensor([ids], dtype=torch.long, device=dev)
