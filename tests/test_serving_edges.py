@@ -1,0 +1,167 @@
+"""Inputs at the edges of the serving operators: values of very unequal size, infinities and NaN that are visible, settings
+out of range, tensors that share memory, forward-mode derivatives, captured restatements."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from titans_pytorch_b200 import ops
+from titans_pytorch_b200.ops.decode_attention import decode_attention_reference
+from titans_pytorch_b200.ops.kv_cache import KINDS, quantise_rows
+
+gpu = pytest.mark.gpu
+HALF = {t: torch.finfo(t).eps / 2 for t in (torch.bfloat16, torch.float16, torch.float32)}
+
+
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs CUDA")
+
+
+def _gen(seed=0, device="cpu"):
+    return torch.Generator(device=device).manual_seed(seed)
+
+
+# ------------------------------------------------------------------------- attention: values of unequal size
+def _sink_case(kind, dtype, d, keys, nats, amplitude, batch=2, heads=2, seed=41):
+    """One key whose score is ``nats`` above the largest other one and whose value row is zero; values of ``amplitude``."""
+    g = _gen(seed)
+    q = (1.5 * torch.randn(batch, heads, d, generator=g)).to(dtype)
+    k = torch.randn(batch, heads, keys, d, generator=g)
+    v = amplitude * torch.randn(batch, heads, keys, d, generator=g)
+    qd = q.double()
+    top = torch.einsum("bhd,bhkd->bhk", qd, k.double()).amax(-1) * d ** -0.5 + nats
+    k[:, :, keys // 3] = (qd * (top / (d ** -0.5 * qd.square().sum(-1)))[..., None]).float()
+    v[:, :, keys // 3] = -0.0
+    (k, ks), (v, vs) = (quantise_rows(x, KINDS[kind]) for x in (k, v))
+    return q.cuda(), ops.KVCache(*(t if t is None else t.cuda() for t in (k, v, ks, vs)))
+
+
+def _sink_bound(q, cache, ref):
+    """|error| of each output element.
+    Scores: d products and sums in fp32 of |q||k| and queries in fp16 (2 d 2^-24 together, as elements below 2^-14 of the
+    row's largest are off by 2^-25 of that), two roundings of a score after that and one of its difference to the
+    maximum (4 * 2^-24 of it); the exponential 2^-20.  Numerator and denominator: twice.
+    Weights: half a step of fp16 (bf16 beside a bf16 cache) of each; in fp16 one that is subnormal by 2^-25, where the
+    largest weight times value scale is 2^7 at least: 2^-32 of that times the stored value.  A row without magnitude has
+    the weight 2^97 at least, so that weights beside it are off by 2^-122 of its own too.
+    Sums of n keys in fp32; the result rounded once.  Steps of subnormals: 2^-149 of an fp32 weight and of the result
+    in fp32, 2^-133 and 2^-24 of a result in bf16 and fp16."""
+    d, n = q.shape[-1], cache.slots
+    k, v, unit, p = cache.k.double(), cache.v.double(), 1.0, None
+    ks = 1.0 if cache.k_scale is None else cache.k_scale.double()[..., None]
+    vs = torch.ones(k.shape[:3], device=k.device, dtype=torch.float64) if cache.v_scale is None else cache.v_scale.double()
+    s = torch.einsum("bhd,bhkd->bhk", q.double(), k * ks) * d ** -0.5
+    p = torch.softmax(s, -1)
+    seen = torch.einsum("bhk,bhkd->bhd", p, (v * vs[..., None]).abs())
+    scores = 2 * d * 2.0 ** -24 * q.double().abs().sum(-1) * (k * ks).abs().amax((-2, -1)) * d ** -0.5 \
+        + 4 * 2.0 ** -24 * s.abs().amax(-1) + 2.0 ** -20
+    exact_bf16 = q.dtype == torch.bfloat16 and cache.v_scale is None
+    half = 0.0 if q.dtype == torch.float32 else HALF[torch.bfloat16] if exact_bf16 else HALF[torch.float16]
+    low = torch.zeros_like(seen)
+    if half and not exact_bf16:
+        # (16-bit caches: of the largest weight, with magnitude or without)
+        sized = v.abs().amax(-1) > 0 if cache.v_scale is not None else torch.ones_like(vs, dtype=torch.bool)
+        unit = (p * vs * sized).amax(-1)
+        low = (2.0 ** -32 * unit[..., None] + (0.0 if cache.v_scale is None else 2.0 ** -122)) * v.abs().sum(-2)
+    return ((2 * scores[..., None] + half + n * 2.0 ** -23) * seen + low) * 1.01 + HALF[q.dtype] * 1.01 * ref.abs() \
+        + 2.0 ** -149 * ((v * vs[..., None]).abs().sum(-2) + 1) \
+        + {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 0.0}[q.dtype]
+
+
+@gpu
+@pytest.mark.parametrize("nats,amplitude", [(10.0, 1.0), (6.0, 1e-2), (4.0, 1e-3), (0.0, 1e-5), (15.0, 1e-4), (25.0, 1.0),
+                                            (90.0, 1.0), (0.0, 1e-28), (2.0, 1e20)])
+@pytest.mark.parametrize("d", [64, 96, 128, 40])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_zero_value_rows_leave_the_other_rows_their_precision(kind, d, nats, amplitude):
+    """A zero row has the scale 1, far above that of small values, and adds nothing."""
+    _cuda()
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        if dtype == torch.float16 and amplitude > 1e4:  # the result does not fit
+            continue
+        for keys in (300, 1100):
+            q, cache = _sink_case(kind, dtype, d, keys, nats, amplitude)
+            n = torch.full((2,), keys, device="cuda")
+            out, lse = ops.decode_attention(q, cache, n, return_lse=True)
+            ref, rl = decode_attention_reference(q.double(), cache, n, scale=d ** -0.5)
+            bad = (out.double() - ref).abs() - _sink_bound(q, cache, ref)
+            assert (bad <= 0).all(), (dtype, keys, float(bad.max()), float(ref.abs().max()))
+            assert ((lse.double() - rl).abs() <= 2.0 ** -14 + 2.0 ** -20 * rl.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("nats", [10.0, 15.0, 20.0])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_zero_value_rows_fp16(d, nats):
+    """fp16 weights beside fp16 keys, in the cache and in a prefix, for few query rows and for many."""
+    _cuda()
+    q, cache = _sink_case("float16", torch.float16, d, 300, nats, 1000.0)
+    n = torch.full((2,), 300, device="cuda")
+    ref, _ = decode_attention_reference(q.double(), cache, n, scale=d ** -0.5)
+    bound = _sink_bound(q, cache, ref)
+    assert ((ops.decode_attention(q, cache, n).double() - ref).abs() <= bound).all()
+    # the first sequence's keys as a prefix, and its query for every row
+    pk, pv = (t[0].transpose(0, 1).contiguous() for t in (cache.k, cache.v))
+    for rows in (3, 40):
+        empty = ops.KVCache.allocate(rows, 2, 8, d, "float16", "cuda")
+        out = ops.decode_attention(q[:1].expand(rows, -1, -1), empty, torch.zeros(rows, dtype=torch.int64, device="cuda"), pk, pv)
+        assert ((out.double() - ref[:1]).abs() <= bound[:1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 96, 128, 40])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_visible_value_rows_that_are_not_finite(kind, d):
+    """They make the output NaN (not zero), and leave the log-sum-exp as it is."""
+    _cuda()
+    g = _gen(43)
+    S, H = 70, 2
+    for dtype in (torch.bfloat16, torch.float32):
+        cache = ops.KVCache.allocate(3, H, S, d, kind, "cuda")
+        new = torch.randn(3, S, H, d, generator=g).to(dtype).cuda()
+        v = torch.randn(3, S, H, d, generator=g).to(dtype).cuda()
+        v[0, :, :, 3] = float("inf")          # every row of the first sequence
+        v[1, 17, 0, 5] = float("nan")         # one row of one head of the second
+        ops.kv_cache_write(cache, new, v, torch.zeros(3, dtype=torch.int64, device="cuda"))
+        q = torch.randn(3, H, d, generator=g).to(dtype).cuda()
+        pk, pv = (torch.randn(5, H, d, generator=g).to(dtype).cuda() for _ in range(2))
+        for lengths in ([1, 18, S], [S, S, 1]):
+            n = torch.tensor(lengths, device="cuda")
+            for prefix in ((None, None), (pk, pv)):
+                out, lse = ops.decode_attention(q, cache, n, *prefix, return_lse=True)
+                ref, rl = decode_attention_reference(q.double(), cache, n, *(None if t is None else t.double() for t in prefix),
+                                                     scale=d ** -0.5)
+                assert torch.equal(torch.isnan(out), torch.isnan(ref))
+                assert torch.isnan(out[0]).all() and torch.isnan(out[1, 0]).all() and torch.isfinite(out[1, 1]).all()
+                assert ((lse.double() - rl).abs() <= 2.0 ** -14).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_value_scales_of_zero_and_infinity(kind):
+    """A cache of the caller's own may hold them: zero adds nothing, whatever the score; infinity is not a number."""
+    _cuda()
+    g = _gen(47)
+    B, H, S, d = 2, 2, 90, 64
+    k, ks = quantise_rows(torch.randn(B, H, S, d, generator=g), KINDS[kind])
+    v, vs = quantise_rows(torch.randn(B, H, S, d, generator=g), KINDS[kind])
+    q = (40 * torch.randn(B, H, d, generator=g)).to(torch.bfloat16).cuda()
+    n = torch.tensor([S, 50], device="cuda")
+    vs[0] = 0.0
+    s = torch.einsum("bhd,bhkd->bhk", q.double().cpu(), k.double() * ks.double()[..., None])[1, :, :50]
+    vs[1].scatter_(1, s.argsort(dim=1, descending=True)[:, :3], 0.0)    # the three likeliest keys of the second
+    cache = ops.KVCache(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    out, lse = ops.decode_attention(q, cache, n, return_lse=True)
+    ref, rl = decode_attention_reference(q.double(), cache, n, scale=d ** -0.5)
+    assert (out[0] == 0).all() and torch.isfinite(out).all() and torch.isfinite(lse).all()
+    assert ((lse.double() - rl).abs() <= 2.0 ** -14 + 2.0 ** -20 * rl.abs()).all()
+    assert ((out.double() - ref).abs() <= 2.0 ** -6 * ref.abs().amax()).all()
+    vs[0, :, 4] = float("inf")
+    cache = ops.KVCache(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    out, lse = ops.decode_attention(q, cache, n, return_lse=True)
+    assert not torch.isfinite(out[0]).any() and torch.isfinite(out[1]).all()
+    assert ((lse.double() - rl).abs() <= 2.0 ** -14 + 2.0 ** -20 * rl.abs()).all()
+
+

@@ -314,11 +314,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps) decode_join_kernel(const floa
 // read them, V registers after the product, so each warp keeps 4 to 8 KB in
 // flight.
 //
-// The running maximum moves only when a score exceeds it by more than 8 (in
-// log2): weights stay below 2^8, and most steps need no exchange between lanes.
+// The running maximum m moves only when a score exceeds it by more than 8 (in
+// log2), so most steps need no exchange between lanes.  Weights are rounded to 16
+// bits for the product (half a step each); sums of them are taken before that, in
+// fp32.  fp16 weights are aimed at 2^7 (exp2(s - m + 7), at most 2^15): what
+// counts 2^-21 of the largest still has all its bits.
+//
 // 8-bit keys and values are exact in fp16; a value's scale is multiplied into its
-// weight.  Weights are rounded to 16 bits for the product (half a
-// step each); sums of them are taken before that, in fp32.
+// weight before that is rounded.  So m follows score + log2(value scale) there.
+// The scale of a row says how large its values are, except where they are all
+// zero (the scale is 1 then, far above that of small values), or where it is no
+// positive number.  Such rows count with kNoLift instead: they move m only as
+// far as keeps their weight, and the sum of 2^20 such, within fp32, and take
+// precision only from what weighs less than 2^-111 of them.  Which rows are zero
+// is looked up in the values only where one of them would move m (64 ragged int8
+// sequences of 12 heads, up to 8192 keys: 129 us with the scale taken as it is, 131 us).
 
 template <typename T> struct Pair;  // two packed 16-bit floats
 template <> struct Pair<__nv_bfloat16> {
@@ -353,6 +363,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
   return d;
 }
+// log2 of the value scale that rows without magnitude count with
+constexpr float kNoLift = -90.f;
+// log2 of what the largest weight is aimed at
+template <typename TM> constexpr float kAim = std::is_same<TM, __half>::value ? 7.f : 0.f;
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -568,7 +583,7 @@ struct Warp {
           lift[u][h] = 0.f;
           if constexpr (k8) {
             vscale[u][h] = vs[u][h];
-            lift[u][h] = __log2f(vs[u][h]);  // -inf behind the end
+            lift[u][h] = fmaxf(__log2f(fabsf(vs[u][h])), kNoLift);  // (kNoLift where it is NaN)
           }
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
@@ -606,6 +621,34 @@ struct Warp {
       const bool more = next < hi, next_whole = next + KEYS <= hi;
       if (more) load_k(next, next_whole);
       if (__any_sync(0xffffffffu, grow > 8.f)) {
+        if constexpr (k8) {  // rows of zeros
+          constexpr uint32_t kMagnitude = std::is_same<C, e4m3>::value ? 0x7f7f7f7fu : 0xffffffffu;  // e4m3 has a -0
+          uint32_t full = 0u;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint32_t any = 0u;
+#pragma unroll
+              for (int j = 0; j < NV * VWP; ++j) any |= vw[u][x][j];
+              full |= (any & kMagnitude) ? 1u << (4 * u + x) : 0u;
+            }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) full |= __shfl_xor_sync(0xffffffffu, full, x);
+          // from the lanes that hold values 2c, 2c + 1, 2c + 8, 2c + 9 to those of scores r, r + 8
+          full = __shfl_sync(0xffffffffu, full, r >> 1);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (!(full >> (4 * u + 2 * h + (r & 1)) & 1u)) {
+                lift[u][h] = kNoLift;
+                // the weight may not fit fp16 (a scale that is not finite stays: the row is none of zeros then)
+                vscale[u][h] = fabsf(vscale[u][h]) < INFINITY ? 0.f : vscale[u][h];
+              } else {
+                lift[u][h] = fminf(lift[u][h], 127.f);  // an infinite scale leaves the weights their sum
+              }
+        }
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -631,7 +674,7 @@ struct Warp {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) use[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e];
+        for (int e = 0; e < 2; ++e) use[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e] - kAim<TM>;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         uint32_t p[NQ][2];
@@ -772,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
       for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
       float* row = mine + (8 * n + 2 * w.c + e) * RS;
       if (w.r == 0) {
-        row[D] = w.m[n][e];
+        row[D] = w.m[n][e] - kAim<TM>;
         row[D + 1] = l;
       }
 #pragma unroll
@@ -964,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) decode_prefix_kerne
           float w[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            w[e] = ex2(sc[n][2 * h + e] - (m[n][e] == -INFINITY ? 0.f : m[n][e]));
+            w[e] = ex2(sc[n][2 * h + e] - (m[n][e] == -INFINITY ? 0.f : m[n][e] - kAim<T>));
             l[n][e] += w[e];
           }
           p[n][h] = transpose8x8(Pair<T>::pack(w[0], w[1]));
@@ -992,7 +1035,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) decode_prefix_kerne
       const int bb = row / a.group, h = hk * a.group + row - bb * a.group;
       float* dst = a.part + (((int64_t)bb * a.Hq + h) * a.splits + a.split0 + split) * (D + 2);
       if (r == 0) {
-        dst[D] = m[n][e];
+        dst[D] = m[n][e] - kAim<T>;
         dst[D + 1] = sum;
       }
 #pragma unroll
