@@ -165,3 +165,34 @@ def test_value_scales_of_zero_and_infinity(kind):
     assert ((lse.double() - rl).abs() <= 2.0 ** -14 + 2.0 ** -20 * rl.abs()).all()
 
 
+# ------------------------------------------------------------------------- the part of a head that is not rotated
+def _tail_case(d, rotary, dtype, device):
+    g = _gen(53)
+    x = torch.randn(2, 3, 4, d, generator=g)
+    if rotary < d:
+        x[0, 0, :, rotary] = float("inf")
+        x[0, 1, :, d - 1] = float("nan")
+        x[1, 0, :, rotary] = -0.0
+        x[1, 1, :, rotary:] = -0.0
+    return x.to(dtype).to(device)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d,rotary", [(96, 20), (64, 2), (64, 8), (128, 64), (96, 94), (20, 6), (96, 48), (64, 0)])
+def test_rope_copies_the_tail(d, rotary, dtype, layout):
+    """Bit for bit, whatever it holds, and without an effect on what is rotated."""
+    _cuda()
+    x = _tail_case(d, rotary, dtype, "cuda")
+    freq = ops.rope_frequencies(max(rotary, 2), device="cuda")[0][:rotary // 2]
+    pos = torch.arange(3, device="cuda") + 7
+    y = ops.rotary_embedding(x, pos, freq, layout=layout)
+    words = torch.int32 if dtype == torch.float32 else torch.int16
+    assert torch.equal(y[..., rotary:].contiguous().view(words), x[..., rotary:].contiguous().view(words))
+    clean = x.clone()
+    clean[..., rotary:] = 1.0
+    assert torch.isfinite(y[..., :rotary]).all()
+    assert torch.equal(y[..., :rotary], ops.rotary_embedding(clean, pos, freq, layout=layout)[..., :rotary])
+
+

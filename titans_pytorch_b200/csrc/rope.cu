@@ -28,8 +28,9 @@ struct RopeArgs {
 
 constexpr int kThreads = 256;
 
-// Interleaved: a 16-byte vector holds whole pairs; the table is padded with
-// (1, 0) past the rotated part, so the copied tail needs no branch.
+// Interleaved: a 16-byte vector holds whole pairs; the table is padded past the
+// rotated part, and what is not rotated there is put back as it was (times (1, 0)
+// an infinity would spoil the other of its pair, and -0 its sign).
 // Half: a work item is a pair of vectors (i, i + n) or one vector of the tail.
 //
 // The vectors are requested before the table is computed, so that the loads
@@ -118,7 +119,14 @@ __global__ void __launch_bounds__(kThreads) rope_vec_kernel(RopeArgs a, int tok_
           u[k] = p0 * c[k / 2] - p1 * n[k / 2];
           u[k + 1] = p0 * n[k / 2] + p1 * c[k / 2];
         }
-        store16<T>(it[q].dst + v * V, u);
+#pragma unroll
+        for (int k = 0; k < V; ++k) y.v[k] = from_f<T>(u[k]);
+        const int live = 2 * a.n - v * V;  // elements of the vector that are rotated
+        if (live < V)
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (k >= live) y.v[k] = x.v[k];
+        *reinterpret_cast<uint4*>(it[q].dst + v * V) = y.raw;
       }
     }
   }
