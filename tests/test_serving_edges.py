@@ -196,3 +196,25 @@ def test_rope_copies_the_tail(d, rotary, dtype, layout):
     assert torch.equal(y[..., :rotary], ops.rotary_embedding(clean, pos, freq, layout=layout)[..., :rotary])
 
 
+@gpu
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,rotary", [(96, 20), (64, 2), (64, 8), (128, 6), (96, 94), (40, 12)])
+def test_cache_write_copies_the_tail(d, rotary, dtype, layout):
+    _cuda()
+    x = _tail_case(d, rotary, dtype, "cuda")
+    freq = ops.rope_frequencies(rotary, device="cuda")[0]
+    start = torch.tensor([0, 5], device="cuda")
+    kind = {torch.bfloat16: "bfloat16", torch.float32: "float32"}[dtype]
+    cache = ops.KVCache.allocate(2, 4, 16, d, kind, "cuda")
+    q = ops.kv_cache_write(cache, x, x, start, q=x, inv_freq=freq, layout=layout)
+    k = torch.stack([cache.k[b, :, int(start[b]):int(start[b]) + 3] for b in range(2)]).transpose(1, 2)
+    words = torch.int32 if dtype == torch.float32 else torch.int16
+    for y in (q, k):
+        tail, want = y[..., rotary:].contiguous(), x[..., rotary:].contiguous()
+        assert torch.equal(torch.isnan(tail), torch.isnan(want))
+        live = ~torch.isnan(want)  # (a NaN may change its payload on the way through fp32)
+        assert torch.equal(tail.view(words)[live], want.view(words)[live])
+        assert torch.isfinite(y[..., :rotary]).all()
+
+

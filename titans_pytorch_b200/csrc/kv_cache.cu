@@ -57,6 +57,7 @@ __device__ __forceinline__ void rotated8(const T* x, int c, const float* cs, con
     table_load(sn + c / 2, b);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
+      if (c + i >= 2 * n) break;  // not times (1, 0): an infinity would spoil the other of its pair
       const float p = v[i], q = v[i + 1];
       v[i] = p * a[i / 2] - q * b[i / 2];
       v[i + 1] = p * b[i / 2] + q * a[i / 2];
