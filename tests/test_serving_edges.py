@@ -218,3 +218,34 @@ def test_cache_write_copies_the_tail(d, rotary, dtype, layout):
         assert torch.isfinite(y[..., :rotary]).all()
 
 
+# ------------------------------------------------------------------------- forward-mode derivatives
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_rope_carries_tangents(device, layout):
+    """The rotation is linear: its directional derivative is the rotation of the direction, with and without a backward."""
+    from torch.autograd import forward_ad
+
+    if device == "cuda":
+        _cuda()
+    freq, amp = ops.rope_frequencies(16, scaling="yarn", factor=4.0, device=device)
+    x, t = (torch.randn(2, 3, 2, 32, generator=_gen(s)).to(device) for s in (59, 61))
+    pos = torch.arange(3, device=device) + 9
+    kw = dict(layout=layout, amplitude=amp)
+    want = ops.rotary_embedding(t, pos, freq, **kw)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with forward_ad.dual_level():
+            y = ops.rotary_embedding(forward_ad.make_dual(leaf, t), pos, freq, **kw)
+            primal, tangent = forward_ad.unpack_dual(y)
+            assert tangent is not None and torch.equal(tangent, want)
+            assert torch.equal(primal, ops.rotary_embedding(x, pos, freq, **kw))
+            with torch.no_grad():
+                assert torch.equal(forward_ad.unpack_dual(ops.rotary_embedding(forward_ad.make_dual(leaf, t), pos, freq, **kw))[1], want)
+    # the tangent of the gradient: of <dy, y> it is zero (y is linear), of |y|^2 / 2 the back-rotated, rotated direction
+    leaf = x.clone().requires_grad_(True)
+    with forward_ad.dual_level():
+        y = ops.rotary_embedding(forward_ad.make_dual(leaf, t), pos, freq, **kw)
+        (g,) = torch.autograd.grad(y.square().sum() / 2, leaf)
+        out = ops.rotary_embedding(forward_ad.unpack_dual(y)[1].detach(), -pos, freq, **kw)
+        assert (forward_ad.unpack_dual(g)[1] - out).abs().max() <= 4 * amp ** 2 * 2.0 ** -20 * float(t.abs().max())
+
+

@@ -15,6 +15,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from ._ext import ext, want_kernels
 
@@ -81,6 +82,7 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, inv_freq, half, amplitude, backward):
         ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
         ctx.args = (half, amplitude, backward)
         return ext().rotary_embedding(x, positions, inv_freq, half, amplitude, backward)
 
@@ -89,6 +91,10 @@ class _RotaryFn(torch.autograd.Function):
         positions, inv_freq = ctx.saved_tensors
         half, amplitude, backward = ctx.args
         return _RotaryFn.apply(dy, positions, inv_freq, half, amplitude, not backward), None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, dx, *_):  # the rotation is linear
+        return _RotaryFn.apply(dx, *ctx.saved_tensors, *ctx.args)
 
 
 def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -99,7 +105,7 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     ``positions``: int64 [T] (shared by the batch) or [B, T]; ``inv_freq``,
     ``amplitude``: from :func:`rope_frequencies`.  ``x`` may have any strides
     (a slice of a fused projection needs no copy); the result is contiguous.
-    Differentiable in ``x``.
+    Differentiable in ``x``, backwards (any number of times) and forwards.
     """
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, not {layout!r}")
@@ -113,7 +119,7 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
         raise ValueError(f"inv_freq must be [n] with 2n <= {x.shape[-1]}, not {tuple(inv_freq.shape)}")
     if want_kernels(x, use_kernels):
         inv_freq = inv_freq.float().contiguous()
-        if x.requires_grad and torch.is_grad_enabled():
+        if (x.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(x).tangent is not None:
             return _RotaryFn.apply(x, positions, inv_freq, layout == "half", float(amplitude), False)
         return ext().rotary_embedding(x, positions, inv_freq, layout == "half", float(amplitude), False)
     return rotary_embedding_reference(x, positions, inv_freq, layout, amplitude)
