@@ -249,3 +249,36 @@ def test_rope_carries_tangents(device, layout):
         assert (forward_ad.unpack_dual(g)[1] - out).abs().max() <= 4 * amp ** 2 * 2.0 ** -20 * float(t.abs().max())
 
 
+# ------------------------------------------------------------------------- the decoders' settings
+def _model(**kw):
+    import titans_pytorch_b200 as T
+
+    torch.manual_seed(0)
+    fields = dict(dim=64, num_heads=2, num_layers=1, vocab_size=128, window_size=8, chunk_size=16, num_persistent_tokens=4,
+                  dropout=0.0, max_seq_len=256, ffn_mult=2.0, memory_hidden_mult=2.0)
+    return T.TitansMAG(T.TitansConfig(**{**fields, **kw})).eval()
+
+
+@pytest.mark.parametrize("dim,heads", [(24, 2), (1024, 2)])
+def test_ring_head_dim_is_checked_before_the_first_step(dim, heads, monkeypatch):
+    """Where the kernels run, head dims that they do not take are refused at once; the restatement takes any."""
+    from titans_pytorch_b200.inference import decode
+
+    model = _model(dim=dim, num_heads=heads)
+    dec = decode.StreamingDecoder(model, kv_cache="int8")
+    assert torch.isfinite(dec.step(torch.zeros(1, 1, dtype=torch.long))).all()
+    monkeypatch.setattr(decode, "want_kernels", lambda t, flag=None: True)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        decode.StreamingDecoder(model, kv_cache="int8")
+
+
+@gpu
+def test_ring_head_dim_is_checked_on_the_gpu():
+    _cuda()
+    from titans_pytorch_b200.inference.decode import StreamingDecoder
+
+    model = _model(dim=24).cuda()
+    with pytest.raises(ValueError, match="multiple of 8"):
+        StreamingDecoder(model, kv_cache="int8")
+
+

@@ -41,10 +41,11 @@ from __future__ import annotations
 import torch
 
 from ..models.memory import MemoryState
+from ..ops._ext import want_kernels
 from ..ops.attention import rope_angles
 from ..ops.conv import conv_silu_norm_reference
 from ..ops.decode_attention import decode_attention
-from ..ops.kv_cache import KINDS, KVCache, kv_cache_write
+from ..ops.kv_cache import HEAD_DIMS, KINDS, KVCache, kv_cache_write
 from ..ops.linear import linear
 from ..ops.memory import activation
 
@@ -76,6 +77,8 @@ class _LayerCache:
         self.P = 0
         if att is not None:
             H, d = att.num_heads, att.head_dim
+            if kv_cache is not None and d not in HEAD_DIMS and want_kernels(att.proj_out.weight, att.use_kernels):
+                raise ValueError(f"kv_cache needs heads of a multiple of 8 dimensions up to {HEAD_DIMS[-1]}, not {d}")
             if kv_cache is None:
                 self.k = torch.zeros(batch, window, H, d, dtype=torch.float32, device=device)
                 self.v = torch.zeros(batch, window, H, d, dtype=torch.float32, device=device)

@@ -25,6 +25,7 @@ from .rope import LAYOUTS, rotary_embedding_reference
 
 KINDS = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16,
          "int8": torch.int8, "fp8": torch.float8_e4m3fn}
+HEAD_DIMS = range(8, 257, 8)  # of a cache that the kernels write and read
 _TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 
 
@@ -32,7 +33,8 @@ class KVCache:
     """Keys and values ``[B, heads, slots, d]`` (and scales ``[B, heads, slots]`` of the 8-bit kinds) of one layer.
 
     The tensors may be views (of a stack of layers, or of part of a batch); a
-    cache object owns no state besides them.
+    cache object owns no state besides them.  On the GPU ``d`` is a multiple of 8
+    from 8 to 256.
     """
 
     __slots__ = ("k", "v", "k_scale", "v_scale")
@@ -172,4 +174,4 @@ def kv_cache_read(cache: KVCache, lengths: torch.Tensor, n: int | None = None, d
     return out[0], out[1]
 
 
-__all__ = ["KVCache", "KINDS", "kv_cache_write", "kv_cache_read", "quantise_rows"]
+__all__ = ["KVCache", "KINDS", "HEAD_DIMS", "kv_cache_write", "kv_cache_read", "quantise_rows"]
