@@ -282,3 +282,57 @@ def test_ring_head_dim_is_checked_on_the_gpu():
         StreamingDecoder(model, kv_cache="int8")
 
 
+class _Uniforms:
+    """Stands for ``sample_tokens`` in the batcher and keeps the numbers that it is given."""
+
+    def __init__(self, monkeypatch):
+        from titans_pytorch_b200.inference import generate
+
+        self.seen, real = [], generate.sample_tokens
+
+        def sample(logits, uniform, **kw):
+            self.seen.append(uniform.clone())
+            return real(logits, uniform, **kw)
+
+        monkeypatch.setattr(generate, "sample_tokens", sample)
+
+
+def _serve(requests, model=None):
+    from titans_pytorch_b200.inference.generate import ContinuousBatcher
+
+    batcher = ContinuousBatcher(model or _model(), max_batch_size=4)
+    for ids, kw in requests:
+        batcher.add_request(ids, **{"max_new_tokens": 4, **kw})
+    return batcher.run()
+
+
+def test_requests_without_a_seed_follow_the_global_one():
+    """``min_p`` alone: the request's numbers follow ``torch.manual_seed``, as those of every other request."""
+    prompt = torch.arange(6)
+    runs = []
+    for seed in (3, 3, 4):
+        torch.manual_seed(seed)
+        model = _model()
+        torch.manual_seed(seed)
+        runs.append([r["ids"].tolist() for r in _serve([(prompt, dict(min_p=1e-6, top_k=0, top_p=1.0)) for _ in range(3)], model)])
+    assert runs[0] == runs[1] and runs[0] != runs[2]
+    assert runs[0][0] != runs[0][1]  # each request has numbers of its own
+
+
+@pytest.mark.parametrize("min_p", [-0.1, 1.5, float("nan")])
+def test_request_min_p_is_checked(min_p):
+    from titans_pytorch_b200.inference.generate import ContinuousBatcher
+
+    for seed in (None, 1):
+        with pytest.raises(ValueError, match="min_p"):
+            ContinuousBatcher(_model()).add_request(torch.arange(3), min_p=min_p, seed=seed)
+
+
+def test_request_top_p_out_of_range_is_the_nearest():
+    """As :func:`sample_next` takes it."""
+    prompt = torch.arange(6)
+    for far, near in ((7.0, 1.0), (-2.0, 0.0)):
+        a, b = (_serve([(prompt, dict(seed=5, top_p=p, top_k=0))])[0]["ids"].tolist() for p in (far, near))
+        assert a == b
+
+

@@ -260,11 +260,14 @@ class ContinuousBatcher:
                     seed: int | None = None) -> int:
         """Queue a request; returns its id.  With a ``seed`` (or ``min_p``) its uniform numbers come from a
         generator of its own, which nothing else served draws from, and all such requests of a step are
-        sampled by one :func:`~titans_pytorch_b200.ops.sampling.sample_tokens` call."""
+        sampled by one :func:`~titans_pytorch_b200.ops.sampling.sample_tokens` call.  Without a ``seed`` that
+        generator is seeded from the global one.  ``top_p`` out of [0, 1] counts as the nearest."""
+        if not 0.0 <= min_p <= 1.0:
+            raise ValueError(f"min_p must be between 0 and 1, not {min_p}")
         uniform = None
         if seed is not None or min_p > 0.0:
             uniform = torch.Generator()
-            uniform.manual_seed(seed) if seed is not None else uniform.seed()
+            uniform.manual_seed(seed if seed is not None else int(torch.randint(0, 2 ** 62, (), device="cpu")))
         rid = self._next_id
         self._next_id += 1
         self.queue.append(dict(id=rid, ids=input_ids.reshape(-1).to(self.device), left=max_new_tokens,
