@@ -336,3 +336,36 @@ def test_request_top_p_out_of_range_is_the_nearest():
         assert a == b
 
 
+def test_uniform_numbers_do_not_follow_the_default_type(monkeypatch):
+    from titans_pytorch_b200.inference.generate import sample_next
+
+    logits = torch.randn(3, 50, generator=_gen(67))
+    want = sample_next(logits, torch.zeros(3, 1, dtype=torch.int64), generator=_gen(1), fused=True)
+    model, prompt = _model(), torch.arange(6)
+    numbers = _Uniforms(monkeypatch)
+    served = _serve([(prompt, dict(seed=5, top_k=0))], model)[0]["ids"].tolist()
+    before = torch.get_default_dtype()
+    for dtype in (torch.float64, torch.bfloat16):
+        try:
+            torch.set_default_dtype(dtype)
+            assert torch.equal(sample_next(logits, torch.zeros(3, 1, dtype=torch.int64), generator=_gen(1), fused=True), want)
+            numbers.seen.clear()
+            assert _serve([(prompt, dict(seed=5, top_k=0))], model)[0]["ids"].tolist() == served
+            assert all(u.dtype == torch.float32 for u in numbers.seen)
+            assert float(numbers.seen[0]) == float(torch.rand((), generator=_gen(5), dtype=torch.float32))
+        finally:
+            torch.set_default_dtype(before)
+
+
+@gpu
+def test_seeded_requests_with_a_default_device():
+    _cuda()
+    model, prompt = _model(dim=128, window_size=16).cuda().to(torch.bfloat16), torch.arange(6)
+    want = _serve([(prompt, dict(seed=5, top_k=0)), (prompt, dict(min_p=0.02))], model)[0]["ids"].tolist()
+    try:
+        torch.set_default_device("cuda")
+        assert _serve([(prompt, dict(seed=5, top_k=0)), (prompt, dict(min_p=0.02))], model)[0]["ids"].tolist() == want
+    finally:
+        torch.set_default_device(None)
+
+

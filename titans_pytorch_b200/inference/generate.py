@@ -62,7 +62,7 @@ def sample_next(logits: torch.Tensor, generated: torch.Tensor, temperature: floa
     from ``generator`` (other tokens than ``torch.multinomial`` would draw from
     the same generator, of the same distribution)."""
     if (fused or min_p > 0.0) and not greedy:
-        u = torch.rand(logits.shape[0], device=logits.device, generator=generator)
+        u = torch.rand(logits.shape[0], dtype=torch.float32, device=logits.device, generator=generator)
         return sample_tokens(logits, u, temperature=max(temperature, 1e-7), top_k=top_k, top_p=min(max(top_p, 0.0), 1.0),
                              min_p=min_p, generated=generated if repetition_penalty != 1.0 else None,
                              repetition_penalty=repetition_penalty)[:, None]
@@ -282,8 +282,9 @@ class ContinuousBatcher:
             return {}
         rs = [self.active[i] for i in rows]
         # one transfer: uniform numbers and settings, a row each
-        host = torch.tensor([[float(torch.rand((), generator=r["uniform"])), max(r["temperature"], 1e-7),
-                              r["top_p"], r["min_p"], float(r["top_k"])] for r in rs], dtype=torch.float32)
+        u = [float(torch.rand((), dtype=torch.float32, device="cpu", generator=r["uniform"])) for r in rs]
+        host = torch.tensor([[a, max(r["temperature"], 1e-7), r["top_p"], r["min_p"], float(r["top_k"])]
+                             for a, r in zip(u, rs)], dtype=torch.float32, device="cpu")
         u, temp, p, m, k = host.to(last.device).unbind(1)
         tok = sample_tokens(last[rows], u.contiguous(), temperature=temp, top_k=k, top_p=p, min_p=m)
         return dict(zip(rows, tok))
