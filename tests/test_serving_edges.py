@@ -369,3 +369,40 @@ def test_seeded_requests_with_a_default_device():
         torch.set_default_device(None)
 
 
+# ------------------------------------------------------------------------- sampling settings out of range
+def _odd_settings(device):
+    nan, inf = float("nan"), float("inf")
+    g = _gen(79)
+    logits = 2 * torch.randn(12, 200, generator=g)
+    u = torch.rand(12, generator=g)
+    odd = dict(top_p=(nan, 2.0, -1.0, inf), min_p=(nan, 3.0, -0.5, -inf))
+    near = dict(top_p=(1.0, 1.0, 0.0, 1.0), min_p=(0.0, 1.0, 0.0, 0.0))
+    for name in odd:
+        for base in (dict(), dict(top_k=30), dict(temperature=0.7, top_p=0.8, min_p=0.01)):
+            a, b = ({**base, name: torch.tensor(v * 3, device=device)} for v in (odd[name], near[name]))
+            yield logits.to(device), u.to(device), u.to(device), a, b
+    # uniform numbers: NaN and negative ones count as 0, those from 1 on give the last token that is kept
+    bad = torch.tensor([nan, -0.3, -inf, 1.0, 1.5, inf] * 2)
+    good = torch.tensor([0.0, 0.0, 0.0] + [1.0 - 2.0 ** -24] * 3).repeat(2)
+    flat = torch.zeros(12, 200)
+    flat[:, :5] = -inf
+    flat[:, 190:] = -inf
+    for kw in (dict(), dict(top_p=0.5), dict(min_p=0.5)):
+        yield flat.to(device), bad.to(device), good.to(device), kw, kw
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_sampling_settings_out_of_range_count_as_the_nearest(device):
+    if device == "cuda":
+        _cuda()
+    for logits, u, v, odd, near in _odd_settings(device):
+        a = ops.sample_tokens(logits, u, return_logprob=True, **odd)
+        b = ops.sample_tokens(logits, v, return_logprob=True, **near)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        assert torch.isfinite(a[1]).all()
+    # a temperature that is NaN: the largest, as 0
+    hot = torch.tensor([float("nan"), 0.0, -1.0] * 4, device=device)
+    tok, lp = ops.sample_tokens(2 * logits + torch.arange(200, device=device) % 7, u, temperature=hot, return_logprob=True)
+    assert (tok == 6).all() and (lp == 0).all()
+
+

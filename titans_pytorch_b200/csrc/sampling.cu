@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   uint2* list = reinterpret_cast<uint2*>(seen_bits + seen_words);
   uint2* first_list = cluster.map_shared_rank(list, 0);
   // all settings at once: each is a memory latency of its own
-  const float temp = a.temp.at(row), pen = a.penalty.at(row), min_p = fminf(a.min_p.at(row), 1.f);
+  const float temp = a.temp.at(row), pen = a.penalty.at(row), min_p = fminf(fmaxf(a.min_p.at(row), 0.f), 1.f);  // NaN: 0
   const double p = (double)a.top_p.at(row), u = (double)a.u[row];
   const int64_t want_k = a.top_k ? a.top_k[row] : a.top_k0;
   const bool greedy = !(temp > 0.f);

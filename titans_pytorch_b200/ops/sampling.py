@@ -56,10 +56,12 @@ def sample_tokens_reference(logits, uniform, temperature, top_k, top_p, min_p, g
     w = torch.where(z >= torch.gather(down, 1, (k - 1)[:, None]), w, torch.zeros_like(w))
     ranked = torch.gather(w, 1, order)
     ahead = torch.cumsum(ranked, dim=1) - ranked
-    nucleus = torch.where(top_p >= 1, torch.full_like(ranked[:, 0], float("inf")), top_p.double() * ranked.sum(dim=1))
+    nucleus = torch.where(top_p < 1, top_p.double() * ranked.sum(dim=1), torch.full_like(ranked[:, 0], float("inf")))
     keep = torch.zeros_like(w, dtype=torch.bool).scatter_(1, order, ahead <= nucleus.clamp(min=0)[:, None])
-    w = torch.where(keep & (w >= min_p.double().clamp(max=1)[:, None]), w, torch.zeros_like(w))
+    min_p = torch.where(min_p > 0, min_p, torch.zeros_like(min_p)).clamp(max=1)
+    w = torch.where(keep & (w >= min_p.double()[:, None]), w, torch.zeros_like(w))
     reach = torch.cumsum(w, dim=1)
+    uniform = torch.where(uniform > 0, uniform, torch.zeros_like(uniform))
     token = (reach <= uniform.double()[:, None] * reach[:, -1:]).sum(dim=1)
     last = torch.where(w > 0, torch.arange(V, device=z.device), -1).amax(dim=1)
     token = torch.minimum(token, last)
@@ -75,7 +77,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
                   use_kernels: bool | None = None):
     """Token ids (int64 [B]) drawn from ``logits`` [B, V] with the numbers ``uniform`` (fp32 [B], in [0, 1)).
 
-    Every setting is a number or a tensor [B]; V is at most 2^19.  ``generated`` (int64 [B, n]):
+    Every setting is a number or a tensor [B]; V is at most 2^19.  In a tensor,
+    ``top_p`` and ``min_p`` out of [0, 1] count as the nearest and NaN as off
+    (``temperature``: as 0); a ``uniform`` below 0 or NaN counts as 0, one from
+    1 on gives the last token that is kept.  ``generated`` (int64 [B, n]):
     tokens that ``repetition_penalty`` applies to; ids outside the vocabulary
     (padding) are passed over.  With ``return_logprob`` also the log-probability
     of each token among those kept (fp32 [B]; 0 where ``temperature <= 0``).
