@@ -406,3 +406,54 @@ def test_sampling_settings_out_of_range_count_as_the_nearest(device):
     assert (tok == 6).all() and (lp == 0).all()
 
 
+# ------------------------------------------------------------------------- the restatement in a captured step
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_cache_write_restatement_leaves_the_rest_as_it_was(kind, device):
+    """Bits of every slot that no new token goes to, NaN among them, with tokens before position 0 and past the counts."""
+    if device == "cuda":
+        _cuda()
+    B, T, H, S, d = 4, 11, 2, 6, 8
+    g = _gen(83)
+    cache = ops.KVCache.allocate(B, H, S, d, kind, device)
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        if t is not None:
+            t.copy_(torch.randn(t.shape, generator=g).to(device))
+    if cache.k_scale is None:
+        cache.k[:, :, 1] = float("nan")
+    old = [t if t is None else t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    k, v = (torch.randn(B, T, H, d, generator=g).to(device) for _ in range(2))
+    start, counts = torch.tensor([-3, 2, 100, -20], device=device), torch.tensor([5, 3, 11, 7], device=device)
+    ops.kv_cache_write(cache, k, v, start, counts=counts, use_kernels=False)
+    bits = {1: torch.uint8, 2: torch.int16, 4: torch.int32}
+    for data, scale, was, scale_was, new in ((cache.k, cache.k_scale, old[0], old[2], k), (cache.v, cache.v_scale, old[1], old[3], v)):
+        row, s = quantise_rows(new, KINDS[kind])
+        for b in range(B):
+            held = {}
+            for t in range(int(counts[b])):
+                p = int(start[b]) + t
+                if p >= 0:
+                    held[p % S] = t
+            for slot in range(S):
+                want = row[b, held[slot]] if slot in held else was[b, :, slot]
+                word = bits[want.element_size()]
+                assert torch.equal(data[b, :, slot].contiguous().view(word), want.contiguous().view(word))
+                if scale is not None:
+                    assert torch.equal(scale[b, :, slot], s[b, held[slot]] if slot in held else scale_was[b, :, slot])
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bfloat16", "int8", "fp8"])
+def test_restatement_decodes_in_a_graph(kind):
+    """A model with ``use_kernels=False`` on the GPU: the captured step of the decoder, with the cache operators in it."""
+    _cuda()
+    from titans_pytorch_b200.inference.decode import StreamingDecoder
+
+    model = _model(dim=128, window_size=16, use_kernels=False).cuda()
+    ids = torch.randint(0, 128, (2, 24), generator=_gen(89)).cuda()
+    a, b = (StreamingDecoder(model, batch=2, graph=g, kv_cache=kind) for g in (False, True))
+    for t in range(ids.shape[1]):
+        x, y = a.step(ids[:, t:t + 1]).float(), b.step(ids[:, t:t + 1]).float()
+        assert torch.isfinite(y).all() and (x - y).norm() <= 1e-4 * x.norm()
+
+

@@ -75,7 +75,7 @@ def quantise_rows(x: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, to
     if dtype not in _TOP:
         return x.to(dtype), None
     x = x.float()
-    top = x.new_tensor(_TOP[dtype])  # a tensor: a Python number would be multiplied by as a reciprocal
+    top = x.new_full((), _TOP[dtype])  # a tensor: a Python number would be multiplied by as a reciprocal
     amax = x.abs().amax(dim=-1)
     bad = ~torch.isfinite(x).all(dim=-1)
     full = (amax >= 2.0 ** -100) & ~bad
@@ -126,23 +126,29 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: torc
 
 
 def _write_reference(cache, k, v, start, counts, q, inv_freq, layout, amplitude, rope_offset):
+    """Reads no value on the host, so that a decoding step with it can be captured."""
     B, H, S, d = cache.k.shape
     T = k.shape[1]
-    t = torch.arange(T, device=k.device)
-    at = start[:, None] + t
+    at = start[:, None] + torch.arange(T, device=k.device)
     kr = k if k.dtype == torch.float64 else k.float()
     if inv_freq is not None:
         kr = rotary_embedding_reference(kr, at + rope_offset, inv_freq, layout, amplitude)
         if q is not None:
             q = rotary_embedding_reference(q, at + rope_offset, inv_freq, layout, amplitude)
-    n = torch.full_like(start, T) if counts is None else counts.clamp(0, T)
-    b, i = torch.nonzero((t < n[:, None]) & (t >= n[:, None] - S) & (at >= 0), as_tuple=True)
-    slot = at[b, i] % S
-    for new, data, scale in ((kr, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
-        stored, s = quantise_rows(new[b, i], data.dtype)
-        data[b, :, slot] = stored
-        if scale is not None:
-            scale[b, :, slot] = s
+    if T:
+        n = torch.full_like(start, T) if counts is None else counts.clamp(0, T)
+        # the newest min(T, S) tokens have a slot each; one that is not stored writes back what its slot held
+        t = n[:, None] - min(T, S) + torch.arange(min(T, S), device=k.device)
+        b, slot = torch.arange(B, device=k.device)[:, None], (start[:, None] + t) % S
+        real = (t >= 0) & (start[:, None] + t >= 0)
+        t = t.clamp(min=0)
+        for new, data, scale in ((kr[b, t], cache.k, cache.k_scale), (v[b, t], cache.v, cache.v_scale)):
+            stored, s = quantise_rows(new, data.dtype)
+            if data.element_size() == 1:  # e4m3 as bytes: not every operation takes it
+                stored, data = stored.view(torch.uint8), data.view(torch.uint8)
+            data[b, :, slot] = torch.where(real[..., None, None], stored, data[b, :, slot])
+            if scale is not None:
+                scale[b, :, slot] = torch.where(real[..., None], s, scale[b, :, slot])
     return None if q is None else q.contiguous()
 
 
