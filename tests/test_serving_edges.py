@@ -457,3 +457,56 @@ def test_restatement_decodes_in_a_graph(kind):
         assert torch.isfinite(y).all() and (x - y).norm() <= 1e-4 * x.norm()
 
 
+# ------------------------------------------------------------------------- tensors that share memory
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_cache_write_of_its_own_rows(device):
+    """New tokens that are views of the cache: what is stored is what they were before the call."""
+    if device == "cuda":
+        _cuda()
+    B, H, S, d = 2, 3, 64, 64
+    freq = ops.rope_frequencies(32, device=device)[0]
+    for kind in ("bfloat16", "float32"):
+        base = [torch.randn(B, H, S, d, generator=_gen(s)).to(KINDS[kind]).to(device) for s in (91, 93)]
+        for shift, T in ((1, 60), (32, 32), (-1, 50)):
+            start = torch.full((B,), 2 + shift, device=device)
+            results = []
+            for own in (True, False):
+                cache = ops.KVCache(*(t.clone() for t in base))
+                k, v = ((t if own else t.clone())[:, :, 2:2 + T].transpose(1, 2)[:, :S - 2 - max(shift, 0)] for t in (cache.k, cache.v))
+                # keys from the values' rows and the other way round too
+                for a, b in ((k, v), (v, k)):
+                    q = ops.kv_cache_write(cache, a, b, start, q=a, inv_freq=freq)
+                    results.append((own, cache.k.clone(), cache.v.clone(), q))
+                    cache.k.copy_(base[0])
+                    cache.v.copy_(base[1])
+            for i in range(2):
+                assert all(torch.equal(x, y) for x, y in zip(results[i][1:], results[2 + i][1:]))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_cache_whose_rows_share_memory_is_not_written(device):
+    """Refused before anything is stored; such a cache can be read."""
+    if device == "cuda":
+        _cuda()
+    S, d = 4, 8
+    one = torch.zeros(1, 2, S, d, device=device)
+    scale = torch.ones(3, 2, S, device=device)
+    k = torch.ones(3, 2, 2, d, device=device)
+    start = torch.zeros(3, dtype=torch.int64, device=device)
+    full = torch.zeros(3, 2, S, d, device=device)
+    eight = full.to(torch.int8)
+    wide = torch.zeros(4 * 2 * S * d, device=device)
+    for cache in (ops.KVCache(one.expand(3, -1, -1, -1), full), ops.KVCache(full, one.expand(3, -1, -1, -1)),
+                  ops.KVCache(full, full), ops.KVCache(wide[:3 * 2 * S * d].view_as(full), wide[2 * S * d:].view_as(full)),
+                  ops.KVCache(eight, eight.clone(), scale[:1].expand(3, -1, -1), scale),
+                  ops.KVCache(eight, eight.clone(), scale, scale)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            ops.kv_cache_write(cache, k, k, start)
+        assert all((t == 0).all() for t in (one, full, eight, wide)) and (scale == 1).all()
+        ops.kv_cache_read(cache, start + 2)
+    # keys and values side by side in one tensor are two caches
+    pair = torch.zeros(3, 2, S, 2 * d, device=device)
+    ops.kv_cache_write(ops.KVCache(pair[..., :d], pair[..., d:]), k, 2 * k, start)
+    assert (pair[:, :, :2, :d] == 1).all() and (pair[:, :, :2, d:] == 2).all() and (pair[:, :, 2:] == 0).all()
+
+

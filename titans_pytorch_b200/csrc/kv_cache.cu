@@ -16,6 +16,8 @@
 // the write takes 110 us, bound by its instructions (rotation, two divisions and
 // eight conversions a lane; memory alone would take 30), the read of 8192 slots
 // 50 us, 75 % of the copy rate.
+#include <ATen/MemoryOverlap.h>
+
 #include "kv_cache.cuh"
 #include "rope.cuh"
 
@@ -213,15 +215,27 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
     if (at[u] < a.n) store8<T>(dst + ((int64_t)blockIdx.y * a.n + at[u]) * a.d + col[u], x[u]);
 }
 
-// `hold` keeps the copy that unaligned rows need.
-Rows rows_of(const at::Tensor& x, at::Tensor& hold, const char* what) {
+// `hold` keeps the copy that unaligned rows need, and rows of the cache itself, which the call overwrites.
+Rows rows_of(const at::Tensor& x, at::Tensor& hold, const at::Tensor& ck, const at::Tensor& cv, const char* what) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 4, what, ": new tokens must be CUDA tensors [B, T, H, d]");
   const at::cuda::CUDAGuard g(x.device());
   const int64_t size = x.element_size();
   const bool fits = x.stride(3) == 1 && x.stride(0) * size % 16 == 0 && x.stride(1) * size % 16 == 0 &&
                     x.stride(2) * size % 16 == 0 && aligned16(x);
-  hold = fits ? x : contig16(x);
+  if (x.is_alias_of(ck) || x.is_alias_of(cv))
+    hold = x.clone(at::MemoryFormat::Contiguous);
+  else
+    hold = fits ? x : contig16(x);
   return Rows{hold.data_ptr(), hold.stride(0), hold.stride(1), hold.stride(2), (int)hold.size(2)};
+}
+
+// Blocks write rows in any order: no two rows may be the same memory.
+void check_distinct(const at::Tensor& a, const at::Tensor& b, const char* what) {
+  using at::MemOverlapStatus;
+  const MemOverlapStatus both = at::get_overlap_status(a, b);
+  TORCH_CHECK(at::has_internal_overlap(a) != at::MemOverlap::Yes && at::has_internal_overlap(b) != at::MemOverlap::Yes &&
+                  both != MemOverlapStatus::Full && both != MemOverlapStatus::Partial,
+              what, ": a cache whose rows share memory cannot be written");
 }
 
 template <typename T, typename C>
@@ -252,9 +266,11 @@ at::Tensor kv_cache_write(at::Tensor& ck, at::Tensor& cv, const c10::optional<at
   a.cv = cache_view(cv, vs, what);
   TORCH_CHECK(ck.sizes() == cv.sizes() && ck.scalar_type() == cv.scalar_type() && ck.device() == cv.device(), what,
               ": the key and value caches must have one shape, type and device");
+  check_distinct(ck, cv, what);
+  if (a.ck.scale) check_distinct(*ks, *vs, what);
   at::Tensor hold_k, hold_v, hold_q;
-  a.k = rows_of(k, hold_k, what);
-  a.v = rows_of(v, hold_v, what);
+  a.k = rows_of(k, hold_k, ck, cv, what);
+  a.v = rows_of(v, hold_v, ck, cv, what);
   const int64_t B = ck.size(0), H = ck.size(1), d = ck.size(3), T = k.size(1);
   TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == B && k.size(2) == H && k.size(3) == d &&
                   k.scalar_type() == v.scalar_type() && k.device() == ck.device() && v.device() == ck.device(),
@@ -273,7 +289,7 @@ at::Tensor kv_cache_write(at::Tensor& ck, at::Tensor& cv, const c10::optional<at
   }
   at::Tensor q_out;
   if (q.has_value() && q->defined()) {
-    a.q = rows_of(*q, hold_q, what);
+    a.q = rows_of(*q, hold_q, ck, cv, what);
     TORCH_CHECK(q->size(0) == B && q->size(1) == T && q->size(3) == d && q->scalar_type() == k.scalar_type() &&
                     q->device() == ck.device(),
                 what, ": q must be [", B, ", ", T, ", heads, ", d, "] of the keys' type and device");

@@ -101,8 +101,10 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: torc
     are stored; positions below 0 are not.  With ``inv_freq`` the keys are
     rotated at position ``start[b] + t + rope_offset`` first, and so is ``q``
     [B, T, query heads, d] if given, which is returned (contiguous, in its own
-    type; as given if there is no ``inv_freq``).  No gradient flows: this is
-    an inference operator.
+    type; as given if there is no ``inv_freq``).  New tokens may be views of the
+    cache: they count as they are before the call.  A cache whose own rows share
+    memory (an expanded tensor, one tensor for keys and values) is refused.  No
+    gradient flows: this is an inference operator.
     """
     B, H, S, d = cache.k.shape
     if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.shape[0] != B or tuple(k.shape[2:]) != (H, d):
@@ -127,6 +129,9 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start: torc
 
 def _write_reference(cache, k, v, start, counts, q, inv_freq, layout, amplitude, rope_offset):
     """Reads no value on the host, so that a decoding step with it can be captured."""
+    for x, y in ((cache.k, cache.v), (cache.k_scale, cache.v_scale)):
+        if x is not None and _shared(x, y):
+            raise RuntimeError("kv_cache_write: a cache whose rows share memory cannot be written")
     B, H, S, d = cache.k.shape
     T = k.shape[1]
     at = start[:, None] + torch.arange(T, device=k.device)
@@ -135,6 +140,7 @@ def _write_reference(cache, k, v, start, counts, q, inv_freq, layout, amplitude,
         kr = rotary_embedding_reference(kr, at + rope_offset, inv_freq, layout, amplitude)
         if q is not None:
             q = rotary_embedding_reference(q, at + rope_offset, inv_freq, layout, amplitude)
+    q = None if q is None else q.clone(memory_format=torch.contiguous_format)
     if T:
         n = torch.full_like(start, T) if counts is None else counts.clamp(0, T)
         # the newest min(T, S) tokens have a slot each; one that is not stored writes back what its slot held
@@ -149,7 +155,16 @@ def _write_reference(cache, k, v, start, counts, q, inv_freq, layout, amplitude,
             data[b, :, slot] = torch.where(real[..., None, None], stored, data[b, :, slot])
             if scale is not None:
                 scale[b, :, slot] = torch.where(real[..., None], s, scale[b, :, slot])
-    return None if q is None else q.contiguous()
+    return q
+
+
+def _shared(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether rows of ``x`` or ``y`` lie in one another, for all that strides tell."""
+    if any(n > 1 and s == 0 for t in (x, y) for n, s in zip(t.shape, t.stride(), strict=True)):
+        return True
+    begin = [t.data_ptr() for t in (x, y)]
+    end = [p + t.numel() * t.element_size() for p, t in zip(begin, (x, y))]
+    return x.is_contiguous() and y.is_contiguous() and x.numel() > 0 and begin[0] < end[1] and begin[1] < end[0]
 
 
 def kv_cache_read(cache: KVCache, lengths: torch.Tensor, n: int | None = None, dtype: torch.dtype = torch.bfloat16,
