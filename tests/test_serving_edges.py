@@ -510,3 +510,19 @@ def test_cache_whose_rows_share_memory_is_not_written(device):
     assert (pair[:, :, :2, :d] == 1).all() and (pair[:, :, :2, d:] == 2).all() and (pair[:, :, 2:] == 0).all()
 
 
+# ------------------------------------------------------------------------- dimensions of size one
+@gpu
+def test_sampling_takes_any_stride_of_a_dimension_of_one():
+    _cuda()
+    logits = torch.randn(1, 40, device="cuda")
+    u = torch.full((1,), 0.5, device="cuda")
+    tokens = torch.tensor([[3, 9, 4]], device="cuda")
+    one = tokens[:, ::2][:, :1]
+    assert one.stride(1) == 2 and one.is_contiguous()
+    kw = dict(repetition_penalty=1.5, return_logprob=True)
+    a, b = (ops.sample_tokens(logits, u, generated=t, **kw) for t in (one, tokens[:, :1].clone()))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    single = logits[:, ::3][:, :1]
+    assert single.stride(1) == 3 and int(ops.sample_tokens(single, u)) == 0
+
+

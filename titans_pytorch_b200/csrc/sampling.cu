@@ -855,7 +855,7 @@ std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const at::Tensor
                                       const c10::optional<at::Tensor>& seen) {
   const char* what = "sample_tokens";
   TB_CHECK_CUDA(logits);
-  TORCH_CHECK(logits.dim() == 2 && logits.stride(1) == 1, what, ": logits must be [B, V] with contiguous rows");
+  TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), what, ": logits must be [B, V] with contiguous rows");
   const int64_t B = logits.size(0), V = logits.size(1);
   TORCH_CHECK(V >= 1 && V <= (1 << 19), what, ": a vocabulary of 1 to 2^19 tokens");
   auto check_rows = [&](const at::Tensor& t, at::ScalarType type, const char* name) {
@@ -894,7 +894,7 @@ std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const at::Tensor
   a.logprob = logprob.data_ptr<float>();
   if (seen.has_value() && seen->defined() && seen->size(1) > 0) {
     TORCH_CHECK(seen->device() == logits.device() && seen->scalar_type() == at::kLong && seen->dim() == 2 &&
-                    seen->size(0) == B && seen->stride(1) == 1 && seen->size(1) < (1ll << 31),
+                    seen->size(0) == B && (seen->stride(1) == 1 || seen->size(1) == 1) && seen->size(1) < (1ll << 31),
                 what, ": generated must be int64 [", B, ", n] with contiguous rows on the logits' device");
     a.seen = seen->data_ptr<int64_t>();
     a.seen_s = seen->stride(0);
