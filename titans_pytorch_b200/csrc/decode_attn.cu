@@ -445,7 +445,6 @@ struct MmaArgs {
   int splits, split0, nsplit;
   int piece;                   // keys of a piece
   int Hq, group, rows, tiles;  // query rows of a key head in this launch; tiles of them
-  int warps_row;               // warps side by side over rows; the others split the keys
   bool shared;                 // rows run over the whole batch (prefix alone)
   float scale_log2;
 };
@@ -731,8 +730,7 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
   const int split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit;
   const int hk = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wr = warp % a.warps_row, wk = warp / a.warps_row, nk = kWarps / a.warps_row;
-  const int row0 = (tile * a.warps_row + wr) * R;
+  const int row0 = tile * R;  // all warps take the same rows and split the keys
   W w;
   w.r = lane >> 2;
   w.c = lane & 3;
@@ -796,14 +794,14 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
     visible(a.cache, b, first, count);
   const int lo = min(split * a.piece, count), hi = min(lo + a.piece, count);
   if constexpr (!CacheTraits<C>::scaled)
-    if (split == 0 && a.ahead.fixed > 0) w.template run<C, false>(a.ahead, 0, hk, 0, 0, (int)a.ahead.fixed, wk, nk);
+    if (split == 0 && a.ahead.fixed > 0) w.template run<C, false>(a.ahead, 0, hk, 0, 0, (int)a.ahead.fixed, warp, kWarps);
   const KeySource& src = a.cache;
   const bool plain = src.k.ss == D && src.v.ss == D && first + hi <= src.S &&
                      (!CacheTraits<C>::scaled || (src.k.qs == 1 && src.v.qs == 1));
   if (plain)
-    w.template run<C, true>(src, a.shared ? 0 : b, hk, first, lo, hi, wk, nk);
+    w.template run<C, true>(src, a.shared ? 0 : b, hk, first, lo, hi, warp, kWarps);
   else
-    w.template run<C, false>(src, a.shared ? 0 : b, hk, first, lo, hi, wk, nk);
+    w.template run<C, false>(src, a.shared ? 0 : b, hk, first, lo, hi, warp, kWarps);
   // O, m and l of the warp's rows to shared memory; lane (r, c) holds queries 2c, 2c + 1
   float* mine = sm + warp * R * RS;
 #pragma unroll
@@ -831,22 +829,24 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
   wait_for_previous();
   __syncthreads();
   // join the warps that split the keys, in their order
-  const int rows = min(a.warps_row * R, a.rows - tile * a.warps_row * R);
+  const int rows = min(R, a.rows - row0);
   for (int i = threadIdx.x; i < rows * D; i += kThreads) {
     const int lr = i / D, e = i - lr * D;
-    const float* p = sm + ((lr / R) * R + lr % R) * RS;  // warps 0 .. warps_row - 1 are the first key part
-    const int step = a.warps_row * R * RS;
+    const float* p = sm + lr * RS;
+    constexpr int step = R * RS;
     float mx = p[D];
-    for (int x = 1; x < nk; ++x) mx = fmaxf(mx, p[x * step + D]);
+#pragma unroll
+    for (int x = 1; x < kWarps; ++x) mx = fmaxf(mx, p[x * step + D]);
     const float use = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f, den = 0.f;
-    for (int x = 0; x < nk; ++x) {
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
       const float f = ex2(p[x * step + D] - use);
       sum += f * p[x * step + e];
       den += f * p[x * step + D + 1];
     }
     int bb, h;
-    place(tile * a.warps_row * R + lr, bb, h);
+    place(row0 + lr, bb, h);
     const int64_t row = (int64_t)bb * a.Hq + h;
     if (a.splits == 1) {
       ((T*)a.out)[row * D + e] = from_f<T>(den == 0.f ? 0.f : sum / den);
@@ -1071,7 +1071,6 @@ void launch_prefix(const MmaArgs& a, int Hkv, int d) {
 // 8 or 16 query rows a warp
 template <typename T, typename C, int D>
 void launch_rows(MmaArgs& a, int Hkv, int B) {
-  a.warps_row = 1;
   a.tiles = (a.rows + 15) / 16;
   if (a.rows <= 8)
     launch_mma<T, C, D, 1>(a, Hkv, B);
