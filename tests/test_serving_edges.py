@@ -526,3 +526,66 @@ def test_sampling_takes_any_stride_of_a_dimension_of_one():
     assert single.stride(1) == 3 and int(ops.sample_tokens(single, u)) == 0
 
 
+# ------------------------------------------------------------------------- what sampling without the operator keeps drawing
+def test_default_sampling_is_the_filtered_multinomial():
+    """``sample_next`` without ``fused`` or ``min_p`` draws what ``torch.multinomial`` draws from the filtered softmax."""
+    from titans_pytorch_b200.inference.generate import sample_next, top_k_filter, top_p_filter
+
+    logits = 3 * torch.randn(4, 90, generator=_gen(71))
+    prompt = torch.randint(0, 90, (4, 7), generator=_gen(72))
+    for seed, temperature, k, p, penalty in ((6, 1.0, 50, 0.9, 1.0), (7, 0.6, 0, 0.8, 1.0), (8, 1.4, 20, 1.0, 1.3)):
+        z = logits / temperature
+        if penalty != 1.0:
+            z = z.clone()
+            for b in range(4):
+                at = prompt[b].unique()
+                z[b, at] = z[b, at] / penalty
+        z = top_p_filter(top_k_filter(z, k), p)
+        want = torch.multinomial(torch.softmax(z, -1), 1, generator=_gen(seed))
+        got = sample_next(logits, prompt, temperature, k, p, penalty, generator=_gen(seed))
+        assert torch.equal(got, want)
+
+
+def test_seeded_request_has_the_same_numbers_whatever_else_is_served(monkeypatch):
+    g = _gen(73)
+    prompts = [torch.randint(0, 128, (6,), generator=g) for _ in range(3)]
+    numbers = _Uniforms(monkeypatch)
+    model = _model()
+    alone = []
+    for i in range(3):
+        numbers.seen.clear()
+        _serve([(prompts[i], dict(seed=100 + i, top_k=0))], model)
+        alone.append(torch.cat(numbers.seen))
+    assert len({tuple(a.tolist()) for a in alone}) == 3
+    numbers.seen.clear()
+    # beside one another, and beside one that draws from the global generator
+    _serve([(prompts[i], dict(seed=100 + i, top_k=0)) for i in range(3)] + [(prompts[0], {})], model)
+    for i in range(3):
+        assert torch.equal(torch.stack([u[i] for u in numbers.seen]), alone[i])
+
+
+@gpu
+@pytest.mark.parametrize("kind,dtype", [("float32", torch.float32), ("float16", torch.float16), ("fp8", torch.float16),
+                                        ("fp8", torch.bfloat16), ("int8", torch.float32), ("bfloat16", torch.float16)])
+@pytest.mark.parametrize("window,d", [(1, 64), (7, 96), (64, 128), (90, 40), (200, 64)])
+def test_window_below_the_ring(kind, dtype, window, d):
+    """Every kind of cache with every kernel that reads it; the visible slots wrap around the ring's end."""
+    _cuda()
+    g = _gen(97)
+    B, Hq, H, S = 6, 4, 2, 96
+    (k, ks), (v, vs) = (quantise_rows(torch.randn(B, H, S, d, generator=g), KINDS[kind]) for _ in range(2))
+    cache = ops.KVCache(*(t if t is None else t.cuda() for t in (k, v, ks, vs)))
+    n = torch.tensor([S + 5, S + 95, 300, 50, 3, 0], device="cuda")
+    q = torch.randn(B, Hq, d, generator=g).to(dtype).cuda()
+    pk, pv = (torch.randn(5, H, d, generator=g).to(dtype).cuda() for _ in range(2))
+    for prefix in ((None, None), (pk, pv)):
+        out, lse = ops.decode_attention(q, cache, n, *prefix, window=window, return_lse=True)
+        wide = [None if t is None else t.double() for t in prefix]
+        ref, rl = decode_attention_reference(q.double(), cache, n, *wide, window=window, scale=d ** -0.5)
+        # scores of order one (|q||k| d^-1/2 2^-24 2 d < 2^-14), weights and queries rounded once, values below 5
+        tol = 5 * (2.0 ** -13 + (0.0 if dtype == torch.float32 else HALF[dtype])) + HALF[dtype] * ref.abs() + 2.0 ** -24
+        assert ((out.double() - ref).abs() <= tol).all()
+        live = torch.isfinite(rl)
+        assert torch.equal(live, torch.isfinite(lse)) and ((lse.double() - rl)[live].abs() <= 2.0 ** -12).all()
+
+
