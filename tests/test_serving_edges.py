@@ -589,3 +589,21 @@ def test_window_below_the_ring(kind, dtype, window, d):
         assert torch.equal(live, torch.isfinite(lse)) and ((lse.double() - rl)[live].abs() <= 2.0 ** -12).all()
 
 
+@gpu
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("factor", [1e-37, 1e-31, 1e31, 1e35])
+def test_queries_of_any_size_beside_8_bit_keys(kind, factor):
+    """bf16 reaches further than the fp16 in which they meet the keys: tiny ones weigh all keys alike, huge ones take one."""
+    _cuda()
+    g = _gen(101)
+    B, H, S, d = 2, 2, 50, 64
+    (k, ks), (v, vs) = (quantise_rows(torch.randn(B, H, S, d, generator=g), KINDS[kind]) for _ in range(2))
+    cache = ops.KVCache(*(t.cuda() for t in (k, v, ks, vs)))
+    n = torch.full((B,), S, device="cuda")
+    q = (factor * torch.randn(B, H, d, generator=g)).to(torch.bfloat16).cuda()
+    out, lse = ops.decode_attention(q, cache, n, return_lse=True)
+    ref, rl = decode_attention_reference(q.double(), cache, n, scale=d ** -0.5)
+    assert ((out.double() - ref).abs() <= 5 * 2.0 ** -10 + 2.0 ** -8 * ref.abs()).all()
+    assert ((lse.double() - rl).abs() <= 2.0 ** -14 + 2.0 ** -14 * rl.abs()).all()
+
+

@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, NQ == 1 ? 3 : 2) decode_mma_kernel(M
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = (__float_as_int(top) >> 23) - 127;
-      if (e > -100 && e < 100) {
+      if (e > -127 && e < 127) {  // both powers are normal numbers
         down = __int_as_float((127 - e) << 23);
         up = __int_as_float((127 + e) << 23);
       }
