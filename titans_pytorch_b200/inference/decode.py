@@ -33,7 +33,10 @@ keeps it in that type instead (half, or a quarter and a scale per token and
 head, of the bytes each step reads): a token is rotated, quantised and stored
 by one kernel (:func:`~titans_pytorch_b200.ops.kv_cache.kv_cache_write`) and the
 step's attention is :func:`~titans_pytorch_b200.ops.decode_attention.decode_attention`,
-which reads the persistent tokens once for the whole batch.
+for which the persistent tokens are stored once for the whole batch.  The
+rotated query and the persistent keys and values are in the model's type there,
+for every ``kv_cache`` (``"float32"`` keeps the ring's own rows in fp32); the
+default ring keeps all of them in fp32.
 """
 
 from __future__ import annotations

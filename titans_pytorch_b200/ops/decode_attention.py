@@ -2,9 +2,16 @@
 
 Every sequence sees the prefix (keys and values that the whole batch shares:
 persistent tokens, a common prompt) and the newest tokens of its own cache.
-The prefix is stored once and read once for the batch, not once per sequence.
+The prefix is stored once.  With 16-bit queries and heads of 64, 96 or 128 it is
+read once for 16 to 128 query rows of the batch; fp32 queries and other heads
+read it once for every sequence, and so does a cache of the queries' type where
+the prefix has at most 128 tokens, which saves a launch.
+
 Softmax statistics and sums are fp32; the result is rounded once to the
-queries' type.  ``csrc/decode_attn.cu`` describes the kernels.
+queries' type.  With 16-bit queries and heads of 64, 96 or 128 the weights are
+rounded to the queries' type before they meet the values (beside an 8-bit cache
+to fp16, as are the queries, scaled by a power of two); elsewhere they stay fp32.
+``csrc/decode_attn.cu`` describes the kernels.
 """
 
 from __future__ import annotations

@@ -5,7 +5,9 @@ Per row, with scalars or one setting per row:
 * ``z = logits / temperature`` in fp32 (then divided by ``repetition_penalty``
   for tokens of ``generated``, whatever their sign, as
   :func:`~titans_pytorch_b200.inference.generate.apply_repetition_penalty`); NaN counts as -inf;
-* weights ``w = exp(z - max z)`` and all sums in fp64;
+* weights ``w = exp(z - max z)`` and all sums in fp64 (the kernel: in integers of 2^-F of the largest weight, with F
+  from 47 up to 2^15 tokens down to 38 at 2^19, whose sums are exact; what weighs less than half a unit is never drawn,
+  and a running sum is off by at most half a unit a token, 2^-33 to 2^-20 of the largest weight);
 * top-k keeps ``z >=`` the k-th largest, ties included (0: off);
 * top-p keeps, in descending order (ties: lower index first), tokens while the
   weight in front of them is at most ``top_p`` of what top-k left (1: off);
